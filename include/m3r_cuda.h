@@ -46,6 +46,9 @@ extern "C" {
  * -> M3R_DTYPE_F16, "bf16" -> M3R_DTYPE_BF16. */
 #define M3R_DTYPE_BF16 0
 #define M3R_DTYPE_F16 1
+/* Further element types of the operators' device buffers. */
+#define M3R_DTYPE_F32 2
+#define M3R_DTYPE_I8 3
 
 /* Output heads.  M3R_HEAD_MAST3R24: the MASt3R DPT + local-feature head, 24-d
  * L2-normalised descriptors (csrc/mps/mpsgraph_engine.mm:383-437; desc_dim 24).
@@ -269,6 +272,137 @@ int m3r_check_checkpoint(const m3r_config* cfg, const char* safetensors_path);
  * Errors: m3r_global_error(). */
 int m3r_match_nn_static(int device, const float* desc_1, const float* desc_2, int64_t n1, int64_t n2, int desc_dim,
                         int32_t* nn_12, int32_t* nn_21, float* best_12, void* stream);
+
+/* ---- operators on device buffers (no reference counterpart; the reference's Precision
+ * enum names int8, core/config.py:42-48, without an implementation).  They are the parts of
+ * a transformer block run in 8-bit integers, for callers that keep their activations on the
+ * device: the row quantiser, the 8-bit product, the residual norm and rotary positions.
+ *
+ * Like m3r_match_nn_static they take DEVICE buffers on `device`, allocate nothing, queue
+ * their work on `stream` (a cudaStream_t, NULL = default stream) and return without waiting,
+ * so they can be captured into a CUDA graph.  The buffers have to stay valid until the
+ * stream's work is done; inputs and outputs must not overlap unless said so.  Sizes and
+ * strides are in elements; a row's elements are contiguous.  Bad arguments return
+ * M3R_ERR_ARG before anything is launched.  Calls that use different output and workspace
+ * buffers may run at the same time, from several threads and on several streams.
+ * Errors: m3r_global_error(). */
+
+/* Rows in 8 bits:  a = max_j |x_ij|,  q_ij = the integer nearest to 127 x_ij / a (ties to
+ * even, exact for every input),  scale_i = a / 127.  A row of zeros has scale 0; a row with an
+ * infinity or a NaN holds zeros and that scale, so that products with it are NaN.
+ * cols <= 16384. */
+typedef struct m3r_quantize_args {
+    int device;
+    int dtype;           /* of x: M3R_DTYPE_BF16, _F16 or _F32 */
+    int64_t rows, cols;
+    int64_t ldx, ldq;    /* row strides; ldq a multiple of 16 to feed m3r_int8_linear */
+    const void* x;
+    int8_t* q;
+    float* scale;        /* [rows] */
+    void* stream;
+} m3r_quantize_args;
+int m3r_quantize_rows(const m3r_quantize_args* args);
+
+#define M3R_ACT_NONE 0
+#define M3R_ACT_GELU 1   /* tanh form (vit_encoder.py:18-20) */
+#define M3R_ACT_RELU 2
+
+/* y[i, n] = act( (sum_k q_ik w_nk) * scale_i * w_scale_n + bias_n ), the sum exact in 32-bit
+ * integers.  x in 16 or 32 bits is quantised row by row first (m3r_quantize_rows; k <= 16384)
+ * into the workspace; x in 8 bits (rows 16-byte aligned, k <= 131072) comes with x_scale.
+ * The weights' rows are 16-byte aligned: w a multiple of 16, ldw a multiple of 16 (pad the
+ * rows of a k that is no multiple of 16; the padding is not used). */
+typedef struct m3r_int8_linear_args {
+    int device;
+    int x_dtype;         /* M3R_DTYPE_BF16, _F16, _F32 or _I8 */
+    int out_dtype;       /* M3R_DTYPE_BF16, _F16 or _F32 */
+    int act;             /* M3R_ACT_* */
+    int64_t rows, n, k;
+    int64_t ldx, ldw, ldo;
+    const void* x;
+    const float* x_scale;  /* [rows], for M3R_DTYPE_I8 only, else NULL */
+    const int8_t* w;       /* [n, k] */
+    const float* w_scale;  /* [n] */
+    const float* bias;     /* [n] or NULL */
+    void* out;             /* [rows, n] */
+    void* workspace;       /* 256-byte aligned, at least m3r_int8_linear_workspace bytes */
+    int64_t workspace_bytes;
+    void* stream;
+} m3r_int8_linear_args;
+int m3r_int8_linear(const m3r_int8_linear_args* args);
+/* Bytes of workspace a call of these sizes needs (0: none), or M3R_ERR_ARG.  Calls that may
+ * run at the same time need a workspace each. */
+int64_t m3r_int8_linear_workspace(int x_dtype, int64_t rows, int64_t n, int64_t k);
+
+#define M3R_NORM_NONE 0
+#define M3R_NORM_LAYER 1  /* (v - mean) / sqrt(var + eps) */
+#define M3R_NORM_RMS 2    /* v / sqrt(mean(v^2) + eps) */
+
+/* The norms before and after a block with its gate and residual scale, in one pass:
+ *   t = y, or N_post(y) * post_weight + post_bias
+ *   r = residual_scale * x + gate * t        (the new residual stream, in x's type)
+ *   h = N(r) * weight + bias                 (the next block's input, from the unrounded r)
+ * h in 16 or 32 bits, or in 8 bits with a scale for each row as m3r_quantize_rows makes it.
+ * NULL: y (r = residual_scale * x; no gate, no post norm then), gate (1), weights (1), biases
+ * (0), r (not written).  r may be x itself.  cols <= 16384. */
+typedef struct m3r_residual_norm_args {
+    int device;
+    int x_dtype, y_dtype;  /* M3R_DTYPE_BF16, _F16 or _F32 */
+    int out_dtype;         /* those or _I8 */
+    int norm, post_norm;   /* M3R_NORM_LAYER or _RMS; post_norm also _NONE */
+    float eps, residual_scale;
+    int64_t rows, cols;
+    int64_t ldx, ldy, ldr, ldo;
+    int64_t rows_per_gate; /* row i takes gate vector i / rows_per_gate; 0: one vector for all */
+    int64_t ld_gate;
+    const void* x;
+    const void* y;
+    const float* gate;
+    const float* post_weight;
+    const float* post_bias;
+    const float* weight;
+    const float* bias;
+    void* r;
+    void* out;
+    float* out_scale;      /* [rows], for M3R_DTYPE_I8 only, else NULL */
+    void* stream;
+} m3r_residual_norm_args;
+int m3r_residual_norm(const m3r_residual_norm_args* args);
+
+/* Rotary positions on the first 2 n_freq of a head's dim values, of one or two tensors
+ * [batch, tokens, heads, dim] (queries and keys):
+ *   (u, v) -> amplitude * (u cos a - v sin a, u sin a + v cos a),  a = position * inv_freq[i]
+ * with pair i at (i, i + n_freq), or at (2 i, 2 i + 1) when interleaved; the values behind are
+ * copied.  Positions are signed integers; angles are reduced in 64 bits, which leaves a position
+ * of 2^31 its angle to 1e-6.  With axes = 2 (n_freq even) the first half of the pairs takes the
+ * positions of axis 0, the second those of axis 1.  out may be x itself, with the same strides. */
+typedef struct m3r_rope_tensor {
+    const void* x;
+    void* out;
+    int64_t heads;                            /* 0: no such tensor */
+    int64_t x_batch, x_token, x_head;         /* element strides */
+    int64_t out_batch, out_token, out_head;
+} m3r_rope_tensor;
+typedef struct m3r_rope_args {
+    int device;
+    int dtype;             /* M3R_DTYPE_BF16, _F16 or _F32 */
+    int interleaved;
+    int axes;              /* 1 or 2 */
+    int pos_bits;          /* 32 or 64: signed integers */
+    float amplitude;
+    int64_t batch, tokens, dim, n_freq;
+    int64_t pos_axis, pos_batch, pos_token;   /* element strides of the positions (0: shared) */
+    const void* positions;
+    const double* inv_freq;                   /* [n_freq], radians a position */
+    m3r_rope_tensor t[2];
+    void* stream;
+} m3r_rope_args;
+int m3r_rope(const m3r_rope_args* args);
+
+/* Waits for the stream and reports a device-side wait of an operator on `device` that ran out
+ * (M3R_ERR_TIMEOUT; the outputs of the calls since are undefined, the context stays usable).
+ * Not to be called during a stream capture. */
+int m3r_operator_status(int device, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -48,6 +48,8 @@ HEAD_DESC_DIM = {HEAD_MAST3R24: 24, HEAD_REF_SIMPLE: 256}
 
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
+DTYPE_F32 = 2         # operator buffers only
+DTYPE_I8 = 3
 DTYPE_NAMES = {DTYPE_BF16: "bf16", DTYPE_F16: "fp16"}
 
 
@@ -103,6 +105,13 @@ SIGNATURES = {
     "m3r_match_nn_static": (_I, [_I, _P, _P, _I64, _I64, _I, _P, _P, _P, _P]),
     "m3r_set_wait_timeout": (_I, [_P, ctypes.c_ulonglong]),
     "m3r_wait_selftest": (_I, [_I, ctypes.c_ulonglong, ctypes.POINTER(_I)]),
+    # the argument structs of the operators travel as packed bytes (ops.py)
+    "m3r_quantize_rows": (_I, [ctypes.c_char_p]),
+    "m3r_int8_linear": (_I, [ctypes.c_char_p]),
+    "m3r_int8_linear_workspace": (_I64, [_I, _I64, _I64, _I64]),
+    "m3r_residual_norm": (_I, [ctypes.c_char_p]),
+    "m3r_rope": (_I, [ctypes.c_char_p]),
+    "m3r_operator_status": (_I, [_I, _P]),
     "m3r_check_checkpoint": (_I, [ctypes.POINTER(M3RConfig), ctypes.c_char_p]),
 }
 

@@ -1,0 +1,460 @@
+"""GPU tests of the operators on device tensors (mast3r_runtime_b200.ops) against plain
+implementations in 64 bits, at the sizes, layouts and values where they can go wrong.
+
+Tolerances count roundings: `half(dtype)` is half a step of the result's type relative to the
+value, U = 2^-24 one 32-bit rounding.  8-bit values and integer sums are compared exactly."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from mast3r_runtime_b200 import ops as o
+
+    return o
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rnd(*shape, seed=0, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+def close(got, want, tol):
+    """|got - want| <= tol everywhere (tol: a tensor of want's shape)."""
+    assert got.shape == want.shape
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float((err - tol).max()):.3e}"
+
+
+# ----------------------------------------------------------------------------- quantize_rows
+def levels(x):
+    """Exact levels and scales: 127 x and (2 n + 1) a are exact in 64 bits, and a quotient of two
+    32-bit values that is no tie is further from it than a 64-bit rounding."""
+    a = x.double().abs().amax(-1, keepdim=True)
+    q = torch.where(a > 0, 127 * x.double() / a, 0).round()
+    return q.to(torch.int8), (a / 127).float().squeeze(-1)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 127), (5, 256), (3, 513), (130, 1000), (67, 1024), (9, 1025),
+                                       (300, 4096), (2, 8200), (3, 16384), (1, 16383)])
+def test_quantize_rows(ops, dtype, rows, cols):
+    x = rnd(rows, cols, seed=rows + cols, dtype=DT[dtype])
+    q, s = ops.quantize_rows(x)
+    wq, wsc = levels(x)
+    assert torch.equal(q, wq)
+    assert torch.equal(s, wsc)
+    assert q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0
+
+
+def test_quantize_ties_and_tiny_magnitudes(ops):
+    # 127 x / a is exactly n + 1/2 for every value (a = 127 * 2^e), and its neighbours
+    a = 127.0
+    v = torch.arange(-126.5, 127, 1.0)
+    near = torch.cat([v, torch.nextafter(v, torch.tensor(1e9)), torch.nextafter(v, torch.tensor(-1e9))])
+    x = torch.cat([near, torch.tensor([a])]).repeat(4, 1)
+    x *= torch.tensor([1.0, 2.0 ** -120, 2.0 ** 100, 2.0 ** -60])[:, None]
+    x = torch.cat([x, torch.zeros(2, x.shape[1])])
+    x[5, 3] = 2.0 ** -149  # the smallest magnitude there is
+    x = x.cuda()
+    q, s = ops.quantize_rows(x)
+    wq, _ = levels(x)
+    assert torch.equal(q, wq)
+    assert int(q[4].abs().max()) == 0 and float(s[4]) == 0 and int(q[5, 3]) == 127
+
+
+def test_quantize_non_finite_rows_and_strides(ops):
+    base = rnd(6, 40, 96, seed=3, dtype=torch.bfloat16)
+    x = base[:, ::2, 8:83]  # rows evenly spaced within a block of 20, not across blocks
+    with pytest.raises(ValueError):
+        ops.quantize_rows(base[:, 1:39:2, :].transpose(0, 1))
+    x = base.view(240, 96)[::3, 5:80]
+    q, s = ops.quantize_rows(x)
+    wq, wsc = levels(x)
+    assert torch.equal(q, wq) and torch.equal(s, wsc)
+    y = rnd(4, 33, seed=4)
+    y[0, 7] = math.inf
+    y[1, 32] = math.nan
+    y[2, 0] = -math.inf
+    y[2, 1] = math.nan
+    q, s = ops.quantize_rows(y)
+    assert int(q[:3].abs().max()) == 0
+    assert math.isinf(s[0]) and math.isnan(s[1]) and math.isnan(s[2])
+    assert torch.equal(q[3], levels(y[3:])[0][0])
+    w = torch.ones(5, 48, dtype=torch.int8, device="cuda")[:, :33]
+    out = ops.int8_linear(y, w, torch.ones(5, device="cuda"), act="relu")
+    assert torch.isnan(out[:3]).all() and torch.isfinite(out[3]).all()
+
+
+# ----------------------------------------------------------------------------- int8_linear
+def ints(rows, k, seed, extreme=False):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.zeros(rows, -(-k // 16) * 16, dtype=torch.int8)
+    q[:, :k] = 127 if extreme else torch.randint(-127, 128, (rows, k), generator=g, dtype=torch.int8)
+    q[:, k:] = 99  # the padding must not count
+    return q.cuda()[:, :k]
+
+
+def act64(y, act):
+    if act == "gelu":
+        return 0.5 * y * (1 + torch.tanh(math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3)))
+    return y.clamp_min(0) if act == "relu" else y
+
+
+def linear64(q, s, w, ws, bias, act, out_dtype):
+    """(value, tolerance): the sum is exact; then one rounding to 32 bits, two scale products, the
+    bias, the activation and the result's type."""
+    p = (q.double() @ w.double().t()) * s.double()[:, None] * ws.double()
+    y = p + (bias.double() if bias is not None else 0)
+    tol = 4 * U * p.abs() + U * y.abs()
+    if act == "gelu":
+        # the derivative of the activation is at most 1.13; its tanh: 2^-11 relative for 16-bit
+        # results, 4 roundings of the argument and the tanh for 32-bit ones
+        t = 2.0 ** -11 + 8 * U if out_dtype is not torch.float32 else 16 * U
+        tol = 1.13 * tol + 0.5 * y.abs() * t + 4 * U * y.abs()
+    z = act64(y, act)
+    # 2^-25: half a step of fp16's smallest values
+    return z, tol + half(out_dtype) * (z.abs() + tol) + 2.0 ** -25
+
+
+SHAPES = [(1, 1, 1), (1, 5, 16), (1, 4096, 1024), (2, 130, 257), (3, 1153, 1000), (7, 64, 4096), (8, 1000, 33),
+          (9, 300, 512), (16, 4096, 640), (17, 129, 2048), (24, 2048, 4096), (33, 520, 128), (64, 1000, 999),
+          (65, 96, 384), (128, 1152, 384), (129, 257, 129), (577, 1153, 1000), (1536, 2304, 768), (2500, 4100, 1040)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("out", ["fp32", "bf16"])
+def test_int8_linear_exact_sums(ops, m, n, k, out):
+    q, w = ints(m, k, m + n), ints(n, k, n + k)
+    s, ws = rnd(m, seed=5).abs() + 0.1, rnd(n, seed=6).abs() * 1e-4
+    y = ops.int8_linear(q, w, ws, x_scale=s, out_dtype=DT[out])
+    want, tol = linear64(q, s, w, ws, None, "none", DT[out])
+    close(y, want, tol)
+
+
+@pytest.mark.parametrize("m", [1, 4, 12, 40, 200, 700])
+@pytest.mark.parametrize("x", DT)
+@pytest.mark.parametrize("out,act,bias", [("fp16", "gelu", True), ("fp32", "gelu", True), ("bf16", "relu", False)])
+def test_int8_linear_quantises_its_rows(ops, m, x, out, act, bias):
+    k, n = 520, 333
+    xs = rnd(m, k, seed=m, dtype=DT[x])
+    if m > 1:
+        xs[-1] = 0  # a row of padding
+    w, ws = ints(n, k, 2), rnd(n, seed=6).abs() * 2e-4
+    b = rnd(n, seed=8) if bias else None
+    y = ops.int8_linear(xs, w, ws, b, act=act, out_dtype=DT[out])
+    q, s = levels(xs)
+    want, tol = linear64(q, s, w, ws, b, act, DT[out])
+    close(y, want, tol)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40, 16384), (5, 130, 131072), (200, 130, 131072)])
+def test_int8_linear_largest_sums(ops, m, n, k):
+    q, w = ints(m, k, 0, extreme=True), ints(n, k, 0, extreme=True)  # sums of 127^2 k, up to 2.1e9
+    one = torch.ones(max(m, n), device="cuda")
+    y = ops.int8_linear(q, w, one[:n], x_scale=one[:m], out_dtype=torch.float32)
+    assert (y.double() - 127.0 ** 2 * k).abs().max() <= U * 127.0 ** 2 * k
+
+
+def test_int8_linear_layouts(ops):
+    """Leading dimensions, strided rows of x, outputs that TMA cannot store, unaligned vectors."""
+    k, n = 256, 77
+    w = ints(n, k, 1)
+    ws = (rnd(n + 1, seed=2).abs() * 1e-3)[1:]
+    b = rnd(n + 1, seed=3)[1:]
+    base = rnd(4, 50, 2 * k, seed=4, dtype=torch.float16)
+    x = base[:, :, k - 3:2 * k - 3]
+    for m in (x, x[:1, :3], x[2, 7]):
+        y = ops.int8_linear(m, w, ws, b, act="none", out_dtype=torch.float32)
+        flat = m.reshape(-1, k)
+        q, s = levels(flat)
+        want, tol = linear64(q, s, w, ws, b, "none", torch.float32)
+        assert y.shape == (*m.shape[:-1], n)
+        close(y.reshape(-1, n), want, tol)
+    assert ops.int8_linear(x[:, :0], w, ws).shape == (4, 0, n)
+
+
+# ----------------------------------------------------------------------------- residual_norm
+def norm64(t, kind, w, b, eps=1e-6):
+    """(value, error of 32-bit statistics): sums of at most 32 values a thread and 10 joins."""
+    mean = t.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(t[..., :1])
+    d = t - mean
+    r = 1 / (d.pow(2).mean(-1, keepdim=True) + eps).sqrt()
+    w = torch.ones_like(t[0]) if w is None else w.double()
+    v = d * r * w
+    err = 64 * U * (v.abs() + t.abs().mean(-1, keepdim=True) * r * w.abs())
+    if b is not None:
+        v = v + b.double()
+    return v, err + U * v.abs(), r * w.abs()
+
+
+def residual64(x, y, gate, alpha, post, pw, pb):
+    r = alpha * x.double()
+    tol = 2 * U * r.abs()
+    if y is not None:
+        t = y.double()
+        et = torch.zeros_like(t)
+        if post:
+            t, et, _ = norm64(t, post, pw, pb)
+        g = torch.ones(1, t.shape[-1], dtype=torch.float64, device=t.device) if gate is None else gate.double()
+        g = g.reshape(-1, t.shape[-1])
+        g = g.repeat_interleave(t.shape[0] // g.shape[0], 0) if g.shape[0] > 1 else g
+        tol = tol + (g * et).abs() + 2 * U * (g * t).abs()
+        r = r + g * t
+    return r, tol + U * r.abs()
+
+
+def check_residual(ops, x, y, w, b, norm, out, **kw):
+    xf, yf = x.reshape(-1, x.shape[-1]), None if y is None else y.reshape(-1, x.shape[-1])
+    want_r, er = residual64(xf, yf, kw.get("gate"), np.float32(kw.get("residual_scale", 1.0)).item(),
+                            kw.get("post_norm"), kw.get("post_weight"), kw.get("post_bias"))
+    r, h = ops.residual_norm(x, y, w, b, norm=norm, out_dtype=out, **kw)
+    # 2^-25: half a step of fp16's smallest values
+    close(r.reshape(want_r.shape), want_r, er + half(x.dtype) * (want_r.abs() + er) + 2.0 ** -25)
+    want_h, eh, slope = norm64(want_r, norm, w, b)
+    # an error e of r moves h by slope e, and through the statistics by at most twice slope max(e) more
+    eh = eh + slope * (er + 2 * (1 + want_h.abs().amax(-1, keepdim=True)) * er.amax(-1, keepdim=True))
+    close(h.reshape(want_r.shape), want_h, eh + half(h.dtype) * (want_h.abs() + eh) + 2.0 ** -25)
+    return r, h
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 33), (4, 256), (7, 384), (130, 1000), (65, 1001), (64, 1024),
+                                       (5, 1032), (301, 4096), (2, 4096), (3, 8191), (2, 16384)])
+@pytest.mark.parametrize("norm,post", [("layer", None), ("rms", "rms"), ("layer", "layer")])
+def test_residual_norm(ops, rows, cols, norm, post):
+    seed = rows * 7 + cols
+    names = list(DT)
+    xd, yd, od = names[seed % 3], names[(seed + 1) % 3], names[(seed // 3) % 3]
+    x, y = rnd(rows, cols, seed=seed, dtype=DT[xd], scale=3), rnd(rows, cols, seed=seed + 1, dtype=DT[yd])
+    w, b = 1 + 0.1 * rnd(cols, seed=1), 0.1 * rnd(cols, seed=2)
+    kw = dict(post_norm=post, post_weight=0.5 + rnd(cols, seed=3).abs(), post_bias=rnd(cols, seed=4)) if post else {}
+    check_residual(ops, x, y, w, b if norm == "layer" else None, norm, DT[od], gate=rnd(cols, seed=5),
+                   residual_scale=0.75, **kw)
+
+
+@pytest.mark.parametrize("stream", DT)
+@pytest.mark.parametrize("branch", DT)
+def test_residual_norm_types_and_gates(ops, stream, branch):
+    x, y = rnd(6, 50, 200, seed=1, dtype=DT[stream]), rnd(6, 50, 200, seed=2, dtype=DT[branch])
+    w = 1 + 0.1 * rnd(200, seed=1)
+    check_residual(ops, x, y, w, None, "rms", DT[branch], gate=rnd(6, 200, seed=5))
+    check_residual(ops, x, None, w, None, "rms", DT[stream], residual_scale=2.0)
+    check_residual(ops, x, y, None, None, "layer", torch.float32)
+    # strided rows, unaligned starts, in place
+    wide = rnd(40, 777, seed=9, dtype=DT[stream])
+    view = wide[::2, 5:405]
+    keep = wide.clone()
+    y2 = rnd(20, 400, seed=3, dtype=DT[branch])
+    r, h = ops.residual_norm(view.clone(), y2, None)
+    r2, h2 = ops.residual_norm(view, y2, None, inplace=True)
+    # rows off the 16-byte grid are summed in another order: both results lie within norm64's
+    # bound of the exact one, so within twice that of each other
+    want, eh, slope = norm64(residual64(r0 := keep[::2, 5:405], y2, None, 1.0, None, None, None)[0], "layer", None, None)
+    er = 2 * U * (r0.double().abs() + y2.double().abs())
+    eh = eh + slope * (er + 2 * (1 + want.abs().amax(-1, keepdim=True)) * er.amax(-1, keepdim=True))
+    assert r2 is view and torch.equal(r2, r)
+    close(h2, h.double(), 2 * (eh + half(h.dtype) * (want.abs() + eh) + 2.0 ** -25))
+    keep[::2, 5:405] = r
+    assert torch.equal(wide, keep)  # nothing beside the rows was written
+
+
+@pytest.mark.parametrize("cols", [64, 1000, 1001, 4096])
+def test_residual_norm_in_8_bits(ops, cols):
+    x, y = rnd(33, cols, seed=1), rnd(33, cols, seed=2, dtype=torch.bfloat16)
+    x[5] = 0
+    y[5] = 0
+    w, b = 1 + 0.1 * rnd(cols, seed=1), None
+    r, h = ops.residual_norm(x, y, w, b, out_dtype=torch.float32)
+    r2, q, s = ops.residual_norm(x, y, w, b, out_dtype=torch.int8)
+    wq, wsc = levels(h)  # the same kernel's 32-bit result, quantised exactly
+    assert torch.equal(r, r2) and torch.equal(q, wq) and torch.equal(s, wsc)
+    assert float(s[5]) == 0 and int(q[5].abs().max()) == 0
+    assert q.stride(0) % 16 == 0
+
+
+# ----------------------------------------------------------------------------- rope
+def rope64(x, pos, f, amplitude, interleaved, axes):
+    """(value, tolerance) for x [batch, tokens, heads, dim], pos [axes, batch or 1, tokens]."""
+    n = f.numel()
+    p = pos.double()
+    a = p[0][..., None] * f
+    if axes == 2:
+        a = torch.cat([p[0][..., None] * f[:n // 2], p[1][..., None] * f[n // 2:]], -1)
+    a = a.unsqueeze(2)
+    c, s = amplitude * a.cos(), amplitude * a.sin()
+    out = x.double().clone()
+    tol = torch.zeros_like(out)
+    i = slice(0, 2 * n, 2) if interleaved else slice(0, n)
+    j = slice(1, 2 * n, 2) if interleaved else slice(n, 2 * n)
+    u, v = x[..., i].double(), x[..., j].double()
+    out[..., i], out[..., j] = u * c - v * s, u * s + v * c
+    # the fraction of a turn in 32 bits (pi U of the angle, as half a turn is pi), 2 steps of sine
+    # and cosine, and 4 roundings of products and sum
+    e = amplitude * (u.abs() + v.abs()) * (math.pi + 4 + 4) * U
+    tol[..., i] = tol[..., j] = e + half(x.dtype) * e
+    tol[..., :2 * n] += half(x.dtype) * out[..., :2 * n].abs() + (2.0 ** -25 if x.dtype is torch.float16 else 0)
+    return out, tol
+
+
+@pytest.mark.parametrize("dim,rot", [(64, 64), (128, 128), (96, 48), (80, 20), (50, 36), (33, 32), (256, 192), (4, 2)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", DT)
+def test_rope(ops, dim, rot, interleaved, dtype):
+    f, amp = ops.rope_frequencies(rot, scaling="by_parts", factor=4.0)
+    for b, t, h, kv in ((1, 1, 3, 1), (2, 37, 4, 2), (3, 211, 1, 5)):
+        q, k = rnd(b, t, h, dim, seed=1, dtype=DT[dtype]), rnd(b, t, kv, dim, seed=2, dtype=DT[dtype])
+        pos = torch.randint(-1000, 1000000, (b, t), generator=torch.Generator().manual_seed(t)).cuda()
+        oq, ok = ops.rope(q, k, pos, f, amplitude=amp, interleaved=interleaved)
+        for x, o in ((q, oq), (k, ok)):
+            want, tol = rope64(x, pos[None], f, amp, interleaved, 1)
+            close(o, want, tol)
+            assert torch.equal(o[..., rot:], x[..., rot:])
+
+
+def test_rope_far_positions_and_shared_ones(ops):
+    f, _ = ops.rope_frequencies(64, scaling="linear", factor=2.0)
+    x = rnd(3, 16, 2, 64, seed=1)
+    far = 2 ** 31 - 17
+    pos = torch.arange(16, dtype=torch.int32).cuda() + (far - 15)
+    o, none = ops.rope(x, None, pos, f)
+    assert none is None
+    want, tol = rope64(x, pos[None, None], f, 1.0, False, 1)
+    # 2^31 turns of 2^-53 relative: 2^-22 / 2 pi of the angle on each side of the comparison
+    tol = tol + (x.abs().amax(-1, keepdim=True) * 2.0 * 2 ** -22).double()
+    close(o, want, tol)
+    o3, _ = ops.rope(x[1], None, pos, f)
+    assert torch.equal(o3, o[1])
+    assert ops.rope(x[:, :0], None, pos[:0], f)[0].shape == (3, 0, 2, 64)
+
+
+def test_rope_two_axes_match_the_models_rotation(ops):
+    """The image tokens' rotation of the model's oracle (rope2d.py:133-146)."""
+    from oracle import model
+
+    f, _ = ops.rope_frequencies(64, base=100.0, axes=2)
+    h, w, heads = 5, 7, 3
+    y, x = torch.meshgrid(torch.arange(h), torch.arange(w), indexing="ij")
+    pos = torch.stack([y.reshape(-1), x.reshape(-1)]).cuda()
+    t = rnd(2, h * w, heads, 64, seed=3)
+    o, _ = ops.rope(t, None, pos, f, axes=2)
+    want, tol = rope64(t, pos[:, None], f, 1.0, False, 2)
+    close(o, want, tol)
+    cos, sin = model.rope_tables(model.positions(h, w), 64)
+    r = model.rope(t.cpu().numpy().astype(np.float64).transpose(0, 2, 1, 3), cos, sin)
+    # the oracle's angles (up to 7: a power, a reciprocal and a product in 32 bits, 6 roundings),
+    # sines and cosines (2) are 32-bit values, and each result has two of them
+    slack = (7 * 6 + 2) * U * 2 * float(t.abs().max())
+    np.testing.assert_allclose(o.cpu().numpy().transpose(0, 2, 1, 3), r, rtol=0, atol=float(tol.max()) + slack)
+
+
+def test_rope_views_planes_and_in_place(ops):
+    f, _ = ops.rope_frequencies(64)
+    b, t, h = 2, 45, 4
+    qkv = rnd(b, t, 3, h, 64, seed=5, dtype=torch.bfloat16)
+    keep = qkv.clone()
+    pos = torch.arange(t, device="cuda")
+    q, k, v = qkv.unbind(2)
+    oq, ok = ops.rope(q, k, pos, f)
+    want, tol = rope64(q, pos[None, None], f, 1.0, False, 1)
+    close(oq, want, tol)
+    planes = [torch.zeros(b, h, t, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ops.rope(q, k, pos, f, out=[p.transpose(1, 2) for p in planes])
+    assert torch.equal(planes[0].transpose(1, 2), oq) and torch.equal(planes[1].transpose(1, 2), ok)
+    assert torch.equal(qkv, keep)
+    iq, ik = ops.rope(q, k, pos, f, inplace=True)
+    assert iq is q and torch.equal(q, oq) and torch.equal(ik, ok) and torch.equal(v, keep[:, :, 2])
+
+
+# ----------------------------------------------------------------------------- streams, graphs, chains
+def block_entry(ops, s):
+    x, h, sc = ops.residual_norm(s["x"], s["y"], s["w"], s["b"], gate=s["gate"], out_dtype=torch.int8)
+    qkv = ops.int8_linear(h, s["wq"], s["ws"], s["bias"], x_scale=sc, out_dtype=torch.float16)
+    q, k, v = qkv.view(2, -1, 3, 4, 64).unbind(2)
+    q, k = ops.rope(q, k, s["pos"], s["f"], axes=2)
+    return x, q, k, v
+
+
+def block_state(ops, seed, grid=(6, 8)):
+    d, t = 256, grid[0] * grid[1]
+    wq, ws = ops.quantize_weight(rnd(3 * d, d, seed=seed, scale=d ** -0.5))
+    yy, xx = torch.meshgrid(torch.arange(grid[0]), torch.arange(grid[1]), indexing="ij")
+    return dict(x=rnd(2 * t, d, seed=seed), y=rnd(2 * t, d, seed=seed + 1, dtype=torch.float16),
+                w=1 + 0.1 * rnd(d, seed=2), b=rnd(d, seed=3), gate=rnd(d, seed=4), wq=wq, ws=ws,
+                bias=rnd(3 * d, seed=5), pos=torch.stack([yy.reshape(-1), xx.reshape(-1)]).cuda(),
+                f=ops.rope_frequencies(64, base=100.0, axes=2)[0])
+
+
+@pytest.mark.parametrize("grid", [(1, 1), (6, 8), (24, 32)])
+def test_block_entry_chain(ops, grid):
+    s = block_state(ops, 11, grid)
+    x, q, k, v = block_entry(ops, s)
+    r, er = residual64(s["x"], s["y"], s["gate"], 1.0, None, None, None)
+    close(x, r, er + half(x.dtype) * r.abs())
+    # from the operator's own 8-bit rows on, the rest is checked exactly as each operator is
+    _, hq, hs = ops.residual_norm(s["x"], s["y"], s["w"], s["b"], gate=s["gate"], out_dtype=torch.int8)
+    want, tol = linear64(hq, hs, s["wq"], s["ws"], s["bias"], "none", torch.float16)
+    shape = (2, -1, 3, 4, 64)
+    close(v, want.view(shape)[:, :, 2], tol.view(shape)[:, :, 2])
+    for i, o in ((0, q), (1, k)):
+        t, e = want.view(shape)[:, :, i], tol.view(shape)[:, :, i]
+        turned, et = rope64(t.half(), s["pos"][:, None], s["f"], 1.0, False, 2)
+        # both halves of a pair carry the product's error and the one of t.half()
+        slack = e + half(torch.float16) * t.abs() + 2.0 ** -25
+        slack = slack + slack.roll(32, -1)
+        close(o, turned, et + slack * (1 + half(torch.float16)))
+
+
+def test_streams_and_graphs(ops):
+    a, b = block_state(ops, 21), block_state(ops, 31)
+    want_a, want_b = block_entry(ops, a), block_entry(ops, b)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):  # two chains at once, each with its own workspace
+        with torch.cuda.stream(s1):
+            ga = block_entry(ops, a)
+        with torch.cuda.stream(s2):
+            gb = block_entry(ops, b)
+        got.append((ga, gb))
+    torch.cuda.synchronize()
+    for ga, gb in got:
+        assert all(torch.equal(i, j) for i, j in zip(ga, want_a)) and all(torch.equal(i, j) for i, j in zip(gb, want_b))
+    graphs = []
+    for s in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = block_entry(ops, s)
+        graphs.append((g, out))
+    for s, seed in ((a, 41), (b, 51)):
+        s["x"].copy_(rnd(*s["x"].shape, seed=seed))
+    want_a, want_b = block_entry(ops, a), block_entry(ops, b)
+    for _ in range(3):
+        for g, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(i, j) for i, j in zip(graphs[0][1], want_a))
+    assert all(torch.equal(i, j) for i, j in zip(graphs[1][1], want_b))
+    ops.status(0)
+
+
+def test_same_inputs_give_the_same_bits(ops):
+    s = block_state(ops, 61)
+    first = block_entry(ops, s)
+    for _ in range(5):
+        assert all(torch.equal(i, j) for i, j in zip(first, block_entry(ops, s)))

@@ -1,0 +1,152 @@
+"""CPU tests of the operators' boundary: the packed argument structs have the C layout, and bad
+arguments are refused before any device work, by the Python functions and by the C ABI."""
+
+from __future__ import annotations
+
+import subprocess
+import textwrap
+
+import pytest
+
+from conftest import ROOT
+
+torch = pytest.importorskip("torch")
+
+
+def test_argument_structs_match_c(tmp_path):
+    from mast3r_runtime_b200 import ops
+
+    src = tmp_path / "layout.c"
+    src.write_text(textwrap.dedent("""
+        #include <stddef.h>
+        #include <stdio.h>
+        #include "m3r_cuda.h"
+        #define P(x) printf("%zu\\n", (size_t)(x))
+        int main(void) {
+          P(sizeof(m3r_quantize_args)); P(offsetof(m3r_quantize_args, scale));
+          P(sizeof(m3r_int8_linear_args)); P(offsetof(m3r_int8_linear_args, workspace_bytes));
+          P(sizeof(m3r_residual_norm_args)); P(offsetof(m3r_residual_norm_args, x));
+          P(sizeof(m3r_rope_args)); P(offsetof(m3r_rope_args, t));
+          return 0;
+        }
+    """))
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    c = list(map(int, subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()))
+    from struct import calcsize
+
+    assert c == [ops._QUANTIZE.size, calcsize("@2i4q2P"), ops._LINEAR.size, calcsize("@4i6q7P"),
+                 ops._RESIDUAL.size, calcsize("@6i2f8q"), ops._ROPE.size, calcsize("@5if7q2P")]
+
+
+def refused(fn, args, text):
+    from mast3r_runtime_b200 import _lib
+
+    lib = _lib.load()
+    assert getattr(lib, fn)(args) == -1, text
+    assert text in lib.m3r_global_error().decode()
+
+
+def test_c_refusals():
+    """Addresses are never dereferenced: every check comes before the first CUDA call."""
+    from mast3r_runtime_b200 import ops
+
+    def quantize(dev=0, dt=0, rows=2, cols=8, ldx=8, ldq=16, x=16, q=16, s=16):
+        return ops._QUANTIZE.pack(dev, dt, rows, cols, ldx, ldq, x, q, s, 0)
+
+    for bad, text in ((dict(dt=3), "must be"), (dict(rows=-1), "rows out of range"), (dict(cols=0), "row length"),
+                      (dict(cols=16385, ldx=16385, ldq=16400), "row length"), (dict(ldx=7), "stride"),
+                      (dict(ldq=7), "stride"), (dict(x=0), "null"), (dict(x=17), "misaligned"),
+                      (dict(rows=2 ** 31), "rows out of range"), (dict(s=18), "misaligned")):
+        refused("m3r_quantize_rows", quantize(**bad), text)
+    refused("m3r_quantize_rows", None, "null")
+
+    def linear(xt=1, ot=1, act=0, m=4, n=32, k=64, ldx=64, ldw=64, ldo=32, x=256, xs=0, w=256, ws=256, b=0, o=256,
+               work=256, size=1 << 20):
+        return ops._LINEAR.pack(0, xt, ot, act, m, n, k, ldx, ldw, ldo, x, xs, w, ws, b, o, work, size, 0)
+
+    for bad, text in ((dict(xt=4), "x must be"), (dict(ot=3), "output must be"), (dict(act=3), "activation"),
+                      (dict(m=-1), "rows out of range"), (dict(n=0), "n out of range"), (dict(k=0), "k out of range"),
+                      (dict(k=16385, ldx=16400, ldw=16400), "k out of range"), (dict(ldw=72), "16-byte aligned"),
+                      (dict(w=264), "16-byte aligned"), (dict(xs=256), "x_scale"), (dict(xt=3), "x_scale"),
+                      (dict(xt=3, xs=256, ldx=72), "16-byte aligned"), (dict(xt=3, xs=256, x=8), "16-byte aligned"),
+                      (dict(work=0), "workspace"), (dict(size=64), "workspace"), (dict(work=320), "workspace"),
+                      (dict(ldo=31), "stride"), (dict(ws=0), "null"), (dict(o=0), "null"), (dict(o=257), "misaligned"),
+                      (dict(b=257), "misaligned"), (dict(xt=3, xs=256, k=131073, ldx=131088, ldw=131088), "k out")):
+        refused("m3r_int8_linear", linear(**bad), text)
+
+    def norm(xt=2, yt=0, ot=0, kind=1, post=0, eps=1e-6, alpha=1.0, rows=4, cols=8, ldx=8, ldy=8, ldr=8, ldo=8, per=0,
+             ldg=0, x=16, y=16, g=0, pw=0, pb=0, w=16, b=16, r=32, o=16, s=0):
+        return ops._RESIDUAL.pack(0, xt, yt, ot, kind, post, eps, alpha, rows, cols, ldx, ldy, ldr, ldo, per, ldg, x, y,
+                                  g, pw, pb, w, b, r, o, s, 0)
+
+    for bad, text in ((dict(xt=3), "x must be"), (dict(yt=3), "y must be"), (dict(ot=4), "output must be"),
+                      (dict(kind=0), "unknown norm"), (dict(post=3), "post norm"), (dict(eps=-1.0), "eps"),
+                      (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"), (dict(y=0, g=16), "without y"),
+                      (dict(pw=16), "post weights"), (dict(o=0), "null"), (dict(ot=3), "out_scale"),
+                      (dict(s=16), "out_scale"), (dict(r=16, ldr=9), "same row stride"), (dict(ldy=4), "stride"),
+                      (dict(g=16, per=2, ldg=4), "stride"), (dict(g=16, per=-1), "negative"), (dict(w=2), "misaligned"),
+                      (dict(cols=16385), "row length")):
+        refused("m3r_residual_norm", norm(**bad), text)
+
+    def rope(dt=0, axes=1, bits=64, b=1, t=4, d=64, n=32, pos=16, f=16, x=16, o=16, h=2, xt=128, ot=128):
+        return ops._ROPE.pack(0, dt, 0, axes, bits, 1.0, b, t, d, n, 0, 0, 1, pos, f, x, o, h, 0, xt, 64, 0, ot, 64,
+                              *(0,) * 9, 0)
+
+    for bad, text in ((dict(dt=3), "values must be"), (dict(axes=3), "axes"), (dict(bits=16), "positions"),
+                      (dict(d=1), "head size"), (dict(n=33), "more frequencies"), (dict(n=0), "more frequencies"),
+                      (dict(axes=2, n=31), "even number"), (dict(b=-1), "batch"), (dict(pos=0), "null"),
+                      (dict(pos=12), "misaligned"), (dict(x=0), "null"), (dict(h=0), "no tensor"),
+                      (dict(h=-1), "heads"), (dict(ot=256), "same strides"), (dict(x=17), "misaligned")):
+        refused("m3r_rope", rope(**bad), text)
+
+
+def test_workspace_sizes():
+    from mast3r_runtime_b200 import _lib
+
+    f = _lib.load().m3r_int8_linear_workspace
+    assert f(3, 100, 64, 64) == 0 and f(0, 0, 64, 64) == 0
+    assert f(1, 1000, 64, 1001) >= 1000 * 1008 + 4000
+    for bad in ((4, 1, 1, 1), (0, -1, 1, 1), (0, 1, 0, 1), (0, 1, 1, 0), (0, 1, 1, 131073)):
+        assert f(*bad) == -1
+
+
+def test_python_refusals():
+    """Tensors on the CPU and wrong shapes or types raise ValueError."""
+    from mast3r_runtime_b200 import ops
+
+    x = torch.zeros(4, 32)
+    w, ws = torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.quantize_rows(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.int8_linear(x, w, ws)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.residual_norm(x, x, None)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.rope(x.view(4, 1, 32), None, torch.arange(4), torch.ones(16, dtype=torch.float64))
+    with pytest.raises(ValueError, match="inv_freq"):
+        ops.rope(x.view(4, 1, 32), None, torch.arange(4), torch.ones(16))
+    with pytest.raises(ValueError, match="n, k"):
+        ops.quantize_weight(torch.zeros(3))
+
+
+def test_rope_frequencies():
+    from mast3r_runtime_b200 import ops
+
+    f, a = ops.rope_frequencies(8, base=10000.0, device="cpu")
+    assert a == 1.0 and f.dtype == torch.float64
+    torch.testing.assert_close(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64))
+    g, _ = ops.rope_frequencies(8, scaling="linear", factor=4.0, device="cpu")
+    torch.testing.assert_close(g, f / 4)
+    g, _ = ops.rope_frequencies(8, scaling="ntk", factor=4.0, device="cpu")
+    torch.testing.assert_close(g[[0, -1]], torch.tensor([1.0, 0.001 / 4], dtype=torch.float64))
+    g, a = ops.rope_frequencies(128, scaling="by_parts", factor=8.0, device="cpu")
+    f, _ = ops.rope_frequencies(128, device="cpu")
+    assert g[0] == f[0] and g[-1] == f[-1] / 8 and a > 1 and bool((g <= f).all()) and bool((g >= f / 8).all())
+    g, _ = ops.rope_frequencies(64, base=100.0, axes=2, device="cpu")
+    assert g.numel() == 32 and torch.equal(g[:16], g[16:]) and abs(float(g[1]) - 100 ** (-1 / 16)) < 1e-12
+    for bad in (dict(rot_dim=7), dict(rot_dim=0), dict(rot_dim=6, axes=2), dict(rot_dim=8, scaling="x"),
+                dict(rot_dim=8, factor=0.5), dict(rot_dim=8, base=0.0), dict(rot_dim=8, axes=3)):
+        with pytest.raises(ValueError):
+            ops.rope_frequencies(**bad, device="cpu")
