@@ -24,6 +24,13 @@ namespace {
 // First wait of any operator kernel that ran out on this device (see mbar_wait).
 __device__ DevStatus g_status;
 
+constexpr int kEpiWarps = 8;
+constexpr int kEpiGroups = kEpiWarps / 4;         // warps that share a TMEM lane quarter
+constexpr int kWarpCols = 256 / kEpiGroups;       // most columns of a tile that one warp handles
+constexpr int kTmaWarp = kEpiWarps;
+constexpr int kMmaWarp = kEpiWarps + 1;
+constexpr int kThreads = (kEpiWarps + 2) * 32;
+
 struct Int8Params {
     int M, N, num_kb, tiles_m, tiles_n;  // tiles_m: blocks of 128 CG rows
     const float* xs;
@@ -40,8 +47,10 @@ struct I8Cfg {
     static constexpr int A_BYTES = 128 * 128;
     static constexpr int B_BYTES = B_ROWS * 128;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int EPI_STAGE_BYTES = kGemmEpiWarps * 4096;
-    static constexpr int FIXED_BYTES = 1024 + EPI_STAGE_BYTES + 256;
+    // each epilogue warp: 4 KB of result rows, and the scale and bias of its columns
+    static constexpr int EPI_STAGE_BYTES = kEpiWarps * 4096;
+    static constexpr int COLS_BYTES = kEpiWarps * kWarpCols * 8;
+    static constexpr int FIXED_BYTES = 1024 + EPI_STAGE_BYTES + COLS_BYTES + 256;
     static constexpr int FIT = (227 * 1024 - FIXED_BYTES) / STAGE_BYTES;
     static constexpr int STAGES = FIT > 8 ? 8 : FIT;
     static constexpr int ACC_COLS = BN;
@@ -60,118 +69,169 @@ __device__ __forceinline__ void tile_at(const Int8Params& p, int t, int& m, int&
     m = group * G + (r - n * gm);
 }
 
-// scale and bias of 32 columns: v = acc * xs * ws + bias, then the activation
-__device__ __forceinline__ void finish32(const Int8Params& p, float (&v)[32], const uint32_t (&acc)[32], float xs,
-                                         int col0) {
-    const bool vec = col0 + 32 <= p.N && (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 &&
-                     (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
-    if (vec) {
-        const float4* w4 = reinterpret_cast<const float4*>(p.ws + col0);
-        const float4* b4 = reinterpret_cast<const float4*>(p.bias + col0);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const float4 w = __ldg(w4 + q);
-            const float4 b = p.bias ? __ldg(b4 + q) : make_float4(0, 0, 0, 0);
-            v[4 * q] = static_cast<float>(static_cast<int>(acc[4 * q])) * xs * w.x + b.x;
-            v[4 * q + 1] = static_cast<float>(static_cast<int>(acc[4 * q + 1])) * xs * w.y + b.y;
-            v[4 * q + 2] = static_cast<float>(static_cast<int>(acc[4 * q + 2])) * xs * w.z + b.z;
-            v[4 * q + 3] = static_cast<float>(static_cast<int>(acc[4 * q + 3])) * xs * w.w + b.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const bool in = col0 + i < p.N;
-            v[i] = static_cast<float>(static_cast<int>(acc[i])) * xs * (in ? __ldg(p.ws + col0 + i) : 0.0f) +
-                   (in && p.bias ? __ldg(p.bias + col0 + i) : 0.0f);
-        }
-    }
-    if (p.act == ACT_GELU) {
-        if (p.out_dt == OP_F32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = gelu_tanh(v[i]);
-        } else {
-            // tanh.approx: relative error 2^-11 of the tanh, below the 16-bit result's rounding
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = gelu_fast(v[i]);
-        }
-    } else if (p.act == ACT_RELU) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];  // keeps NaN
-    }
+// Pairs of 32-bit values in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
-// One tile's rows of this thread (tile row r), column group grp: units of 128 output bytes
-// a row (32 fp32 or 64 16-bit columns), staged in shared memory and stored by TMA, or by
-// row-contiguous thread stores where the output's layout does not allow TMA.
-template <int BN>
+constexpr float kGelu0 = 0.7978845608028654f;             // sqrt(2 / pi)
+constexpr float kGelu1 = 0.7978845608028654f * 0.044715f;
+
+__device__ __forceinline__ float tanh_approx(float x) {
+    float t;
+    asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(x));
+    return t;
+}
+
+// x / 2 (1 + tanh u) = x / (1 + exp(-2 u)), to a few 32-bit roundings
+__device__ __forceinline__ float gelu_f32(float x, float u) {
+    return x * __frcp_rn(1.0f + ex2_approx(-2.885390081777927f * u));
+}
+
+// Two neighbouring columns of a row: acc * xs * ws + bias, then the activation.
+template <int OUT, int ACT>
+__device__ __forceinline__ uint64_t finish2(uint32_t a0, uint32_t a1, float xs, const ulonglong2& col) {
+    uint64_t v = fma2(mul2(pair(static_cast<int>(a0), static_cast<int>(a1)), pair(xs, xs)), col.x, col.y);
+    if constexpr (ACT == ACT_GELU) {
+        const float2 u = unpair(mul2(v, fma2(mul2(v, v), pair(kGelu1, kGelu1), pair(kGelu0, kGelu0))));
+        if constexpr (OUT == OP_F32) {
+            const float2 x = unpair(v);
+            v = pair(gelu_f32(x.x, u.x), gelu_f32(x.y, u.y));
+        } else {
+            // tanh.approx: relative error 2^-11 of the tanh, below the 16-bit result's rounding
+            const uint64_t x = mul2(v, pair(0.5f, 0.5f));
+            v = fma2(x, pair(tanh_approx(u.x), tanh_approx(u.y)), x);
+        }
+    } else if constexpr (ACT == ACT_RELU) {
+        const float2 x = unpair(v);
+        v = pair(x.x < 0.0f ? 0.0f : x.x, x.y < 0.0f ? 0.0f : x.y);  // keeps NaN
+    }
+    return v;
+}
+
+// Four 8 x 8 blocks of 16-bit values in fragment order to shared memory: lane l gives the address of
+// row l % 8 of block l / 8.
+__device__ __forceinline__ void store_blocks(const void* row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a),
+                 "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+
+template <int OUT>
+struct OutType {
+    using T = __half;
+};
+template <>
+struct OutType<OP_BF16> {
+    using T = __nv_bfloat16;
+};
+
+// One tile's 32 rows of a warp (from global row `row0`), column group grp: units of 128 output
+// bytes a row (32 fp32 or 64 16-bit columns), staged in shared memory and stored by TMA, or by
+// row-contiguous thread stores where the output's layout does not allow TMA.  The sums come from
+// TMEM as fragments -- a thread has 2 columns of every 8, of 4 rows -- so that a column's scale and
+// bias go to the 4 threads that need them: with a whole row a thread, broadcasting every column's
+// 8 bytes to 32 threads took more shared-memory time than all else.  cols: (scale 2, bias 2) of the
+// warp's column pairs; xs: the scales of the thread's rows 8 i + lane / 4.  `release` hands the
+// accumulator back once the last of it is in registers.
+template <int BN, int OUT, int ACT, class Release>
 __device__ __forceinline__ void i8_epilogue(const Int8Params& p, const CUtensorMap* map_out, uint32_t tacc,
-                                            long long row0, int r, int grp, int n0, const RowStage& st) {
-    const long long grow = row0 + r;
-    const bool valid = grow < p.M;
-    const bool wok = grow - st.lane < p.M;  // the warp's first row exists
-    const float xs = valid ? __ldg(p.xs + grow) : 0.0f;
-    const int unit = p.out_dt == OP_F32 ? 32 : 64;
+                                            long long row0, int grp, int n0, const RowStage& st,
+                                            const ulonglong2* cols, const float (&xs)[4], Release&& release) {
+    constexpr int unit = OUT == OP_F32 ? 32 : 64;
+    constexpr int esz = OUT == OP_F32 ? 4 : 2;
+    const int lane = st.lane;
+    const int end = min(BN, p.N - n0);
+    if (grp * unit >= end) release();
+    cols += lane & 3;
 #pragma unroll 1
-    for (int c0 = grp * unit; c0 < BN; c0 += 2 * unit) {
+    for (int c0 = grp * unit; c0 < end; c0 += kEpiGroups * unit, cols += unit / 2) {
         const int col0 = n0 + c0;
-        if (col0 >= p.N) break;  // warp-uniform
-        uint4 o[8];
-        {
-            uint32_t raw[32];
-            float v[32];
-            tmem_ld32(tacc + c0, raw);
-            tmem_wait_ld();
-            finish32(p, v, raw, xs, col0);
-            if (p.out_dt == OP_F32) {
+        uint32_t lo[unit / 2], hi[unit / 2];  // rows 0-15 and 16-31
+        if constexpr (OUT == OP_F32) {
+            tmem_ld_frag4(tacc + c0, lo);
+            tmem_ld_frag4(tacc + (16u << 16) + c0, hi);
+        } else {
+            tmem_ld_frag8(tacc + c0, lo);
+            tmem_ld_frag8(tacc + (16u << 16) + c0, hi);
+        }
+        if (p.c_tma && lane == 0) bulk_wait_read_all();
+        tmem_wait_ld();
+        if (c0 + kEpiGroups * unit >= end) release();
+        __syncwarp();  // the previous unit's reads of the stage (threads or TMA) are done
+        if constexpr (OUT == OP_F32) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    o[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),
-                                      __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
-            } else {
-                float hi[32];
-                tmem_ld32(tacc + c0 + 32, raw);
-                tmem_wait_ld();
-                finish32(p, hi, raw, xs, col0 + 32);
-                if (p.out_dt == OP_F16)
-                    pack16x64<__half>(o, v, hi);
-                else
-                    pack16x64<__nv_bfloat16>(o, v, hi);
+            for (int g = 0; g < 4; ++g) {
+                const ulonglong2 c = cols[4 * g];
+                const uint64_t v[4] = {finish2<OUT, ACT>(lo[4 * g], lo[4 * g + 1], xs[0], c),
+                                       finish2<OUT, ACT>(lo[4 * g + 2], lo[4 * g + 3], xs[1], c),
+                                       finish2<OUT, ACT>(hi[4 * g], hi[4 * g + 1], xs[2], c),
+                                       finish2<OUT, ACT>(hi[4 * g + 2], hi[4 * g + 3], xs[3], c)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    reinterpret_cast<uint64_t*>(st.at(8 * i + (lane >> 2), 2 * g + ((lane & 3) >> 1)))[lane & 1] = v[i];
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 8; g += 2) {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const ulonglong2 c = cols[4 * (g + e)];
+                    const uint32_t* l = lo + 4 * (g + e);
+                    const uint32_t* h = hi + 4 * (g + e);
+                    const float2 v[4] = {unpair(finish2<OUT, ACT>(l[0], l[1], xs[0], c)),
+                                         unpair(finish2<OUT, ACT>(l[2], l[3], xs[1], c)),
+                                         unpair(finish2<OUT, ACT>(h[0], h[1], xs[2], c)),
+                                         unpair(finish2<OUT, ACT>(h[2], h[3], xs[3], c))};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[4 * e + i] = Elem<typename OutType<OUT>::T>::pack(v[i].x, v[i].y);
+                }
+                // blocks: rows 0-7 and 8-15 (then 16-23 and 24-31) of column groups g and g + 1
+                const int row = (lane & 7) + (lane & 8), chunk = g + (lane >> 4);
+                store_blocks(st.at(row, chunk), w[0], w[1], w[4], w[5]);
+                store_blocks(st.at(row + 16, chunk), w[2], w[3], w[6], w[7]);
             }
         }
-        if (p.c_tma && st.lane == 0) bulk_wait_read_all();
-        __syncwarp();  // the previous unit's reads of the stage (threads or TMA) are done
-        st.put_own(o);
         if (p.c_tma) {
             fence_proxy_async_smem();
             __syncwarp();
-            if (st.lane == 0 && wok) {
-                tma_store_2d(map_out, st.buf, col0, static_cast<int>(grow));
+            if (lane == 0 && row0 < p.M) {
+                tma_store_2d(map_out, st.buf, col0, static_cast<int>(row0));
                 bulk_commit();
             }
         } else {
             __syncwarp();
-            const int esz = p.out_dt == OP_F32 ? 4 : 2;
+            // element accesses, a row's 128 bytes by 32 lanes: any alignment, whole sectors
             const int bytes = (col0 + unit <= p.N ? unit : p.N - col0) * esz;
-            char* dst = valid ? static_cast<char*>(p.out) + (grow * p.ldo + col0) * esz : nullptr;
-            const int c = st.lane & 7;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = i * 4 + (st.lane >> 3);
-                char* d = reinterpret_cast<char*>(
-                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
-                const uint4 u = *st.at(row, c);
-                if (d == nullptr) continue;
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-                if (esz == 4) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c * 16 + 4 * e < bytes) *reinterpret_cast<uint32_t*>(d + c * 16 + 4 * e) = w[e];
+            const int rows = static_cast<int>(min(32LL, p.M - row0));
+            char* d = static_cast<char*>(p.out) + (row0 * p.ldo + col0) * esz + lane * 4;
+#pragma unroll 4
+            for (int row = 0; row < rows; ++row, d += p.ldo * esz) {
+                const uint32_t u = reinterpret_cast<const uint32_t*>(st.at(row, lane >> 2))[lane & 3];
+                if (lane * 4 >= bytes) continue;
+                if constexpr (esz == 4) {
+                    *reinterpret_cast<uint32_t*>(d) = u;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c * 16 + 2 * e < bytes)
-                            *reinterpret_cast<uint16_t*>(d + c * 16 + 2 * e) =
-                                static_cast<uint16_t>(w[e >> 1] >> ((e & 1) * 16));
+                    *reinterpret_cast<uint16_t*>(d) = static_cast<uint16_t>(u);
+                    if (lane * 4 + 2 < bytes) *reinterpret_cast<uint16_t*>(d + 2) = static_cast<uint16_t>(u >> 16);
                 }
             }
         }
@@ -181,7 +241,7 @@ __device__ __forceinline__ void i8_epilogue(const Int8Params& p, const CUtensorM
 // CG = 2: launched as clusters of 2 CTAs; the even CTA's thread issues the M = 256 MMAs.  A
 // wait that runs out raises the abort flag of both CTAs; neither leaves before the other.
 template <int BN, int CG>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                      const __grid_constant__ CUtensorMap mapC, const __grid_constant__ Int8Params p) {
     using C = I8Cfg<BN, CG>;
@@ -191,7 +251,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint8_t* sA = smem;
     uint8_t* sB = smem + STAGES * C::A_BYTES;
     uint8_t* epi_stage = smem + STAGES * C::STAGE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(epi_stage + C::EPI_STAGE_BYTES);
+    uint8_t* epi_cols = epi_stage + C::EPI_STAGE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(epi_cols + C::COLS_BYTES);
     uint64_t* full = bars;
     uint64_t* empty = bars + STAGES;
     uint64_t* tfull = bars + 2 * STAGES;
@@ -209,14 +270,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int num_units = gridDim.x / CG;
     const int num_tiles = p.tiles_m * p.tiles_n;
 
-    if (warp == kGemmTmaWarp && lane == 0) {
+    if (warp == kTmaWarp && lane == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], CG * kGemmEpiWarps);
+            mbar_init(&tempty[b], CG * kEpiWarps);
         }
         mbar_init(mma_done, 1);
         *abort_flag = 0;
@@ -224,7 +285,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         prefetch_tmap(&mapA);
         prefetch_tmap(&mapB);
     }
-    if (warp == kGemmMmaWarp) {
+    if (warp == kMmaWarp) {
         if (CG == 2)
             tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
         else
@@ -246,7 +307,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (CG == 2) st_cluster_u32(peer_abort_c, 1u);
     };
 
-    if (warp == kGemmTmaWarp) {
+    if (warp == kTmaWarp) {
         if (lane == 0) {
             uint32_t it = 0;
             bool ok = true;
@@ -290,7 +351,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 }
             }
         }
-    } else if (warp == kGemmMmaWarp) {
+    } else if (warp == kMmaWarp) {
         if (lane == 0 && leader) {
             constexpr uint32_t idesc = idesc_i8kind(128 * CG, BN);
             uint32_t it = 0, tcount = 0;
@@ -348,27 +409,71 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int quarter = warp & 3;
         const int grp = warp >> 2;
         const RowStage st{epi_stage + warp * 4096, lane};
+        float4* const cols = reinterpret_cast<float4*>(epi_cols + warp * kWarpCols * 8);  // (scale 2, bias 2)
         uint32_t tcount = 0;
         for (int t = unit; t < num_tiles; t += num_units, ++tcount) {
             const uint32_t buf = tcount & 1;
             int m, n;
             tile_at(p, t, m, n);
+            const long long row0 = static_cast<long long>(m * CG + rank) * 128 + quarter * 32;  // of the warp
+            // the scales and biases of the tile, before its sums are there: lane l brings columns
+            // 2 l and 2 l + 1 of each 64 that the warp handles, unit by unit
+            __syncwarp();  // the previous tile's reads are done
+#pragma unroll
+            for (int j = 2 * lane; j < kWarpCols; j += 64) {
+                const int c = n * BN + (p.out_dt == OP_F32 ? (grp + (j >> 5) * kEpiGroups) * 32 + (j & 31)
+                                                           : (grp + (j >> 6) * kEpiGroups) * 64 + (j & 63));
+                float4 q = make_float4(0, 0, 0, 0);
+                if (c < p.N) {
+                    q.x = __ldg(p.ws + c);
+                    if (p.bias) q.z = __ldg(p.bias + c);
+                }
+                if (c + 1 < p.N) {
+                    q.y = __ldg(p.ws + c + 1);
+                    if (p.bias) q.w = __ldg(p.bias + c + 1);
+                }
+                cols[j >> 1] = q;
+            }
+            __syncwarp();
+            float xs[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const long long r = row0 + 8 * i + (lane >> 2);
+                xs[i] = r < p.M ? __ldg(p.xs + r) : 0.0f;
+            }
             if (!mbar_wait(&tfull[buf], (tcount >> 1) & 1, abort_flag, kDevTimeoutEpilogue, err)) {
                 abort_pair();
                 break;
             }
             tc_fence_after();
             const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * C::ACC_COLS;
-            i8_epilogue<BN>(p, &mapC, tacc, static_cast<long long>(m * CG + rank) * 128, quarter * 32 + lane, grp,
-                            n * BN, st);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (CG == 2)
-                    mbar_arrive_cluster(tempty_c + buf * 8);
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2)
+                        mbar_arrive_cluster(tempty_c + buf * 8);
+                    else
+                        mbar_arrive(&tempty[buf]);
+                }
+            };
+            // one copy of the epilogue for each result type and activation
+            auto by_act = [&](auto out) {
+                constexpr int OUT = decltype(out)::value;
+                const ulonglong2* cl = reinterpret_cast<const ulonglong2*>(cols);
+                if (p.act == ACT_GELU)
+                    i8_epilogue<BN, OUT, ACT_GELU>(p, &mapC, tacc, row0, grp, n * BN, st, cl, xs, release);
+                else if (p.act == ACT_RELU)
+                    i8_epilogue<BN, OUT, ACT_RELU>(p, &mapC, tacc, row0, grp, n * BN, st, cl, xs, release);
                 else
-                    mbar_arrive(&tempty[buf]);
-            }
+                    i8_epilogue<BN, OUT, ACT_NONE>(p, &mapC, tacc, row0, grp, n * BN, st, cl, xs, release);
+            };
+            if (p.out_dt == OP_F32)
+                by_act(std::integral_constant<int, OP_F32>());
+            else if (p.out_dt == OP_F16)
+                by_act(std::integral_constant<int, OP_F16>());
+            else
+                by_act(std::integral_constant<int, OP_BF16>());
         }
         if (lane == 0) bulk_wait_all();  // TMA stores of this warp complete before the CTA ends
     }
@@ -377,7 +482,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         cluster_sync();
     else
         __syncthreads();
-    if (warp == kGemmMmaWarp) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         if (CG == 2)
             tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
@@ -434,7 +539,7 @@ void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long lo
     const int max_units = sm_count(dev) / CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CG * (units < max_units ? units : max_units));
-    cfg.blockDim = dim3(kGemmThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::SMEM_BYTES;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];

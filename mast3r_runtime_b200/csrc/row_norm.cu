@@ -201,60 +201,86 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH>& s, RowReduce
     }
 }
 
-// The integer nearest to 127 v / a, ties to even.  p = v * inv is within 2e-5 of it (two
-// roundings of a value up to 127); where that leaves open on which side of a half it lies,
-// the two exact products 254 v and (2 m + 1) a decide.
-__device__ __forceinline__ int quantize_value(float v, float pre, float inv, float a) {
-    const float p = v * pre * inv;
-    const float m = rintf(p);
-    if (fabsf(p - m) > 0.49997f) {
-        const float lo = floorf(p);
-        const double d = 254.0 * static_cast<double>(v) - (2.0 * static_cast<double>(lo) + 1.0) * static_cast<double>(a);
-        const int l = static_cast<int>(lo);
-        return d > 0.0 ? l + 1 : d < 0.0 ? l : (l & 1) ? l + 1 : l;
+// The integer nearest to 127 v / a, ties to even, decided by the two exact products 254 v and
+// (2 m + 1) a on either side of a half.
+__device__ __noinline__ int quantize_exact(float v, float p, float a) {
+    const float lo = floorf(p);
+    const double d = 254.0 * static_cast<double>(v) - (2.0 * static_cast<double>(lo) + 1.0) * static_cast<double>(a);
+    const int l = static_cast<int>(lo);
+    return d > 0.0 ? l + 1 : d < 0.0 ? l : (l & 1) ? l + 1 : l;
+}
+
+// Eight values in 8 bits.  p = v * inv lies within 2e-5 of 127 v / a (two roundings of a value up
+// to 127), so that its nearest integer is the right one unless p is that near to a half: one test
+// for the eight, taken for about one value in 10^5, sends them to quantize_exact.  Adding 1.5 * 2^23
+// rounds p to the integer that then stands in the sum's low byte.
+__device__ __forceinline__ uint2 quantize8(const float* v, float pre, float inv, float a) {
+    constexpr float kMagic = 12582912.0f;
+    float t[8], off = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float p = v[j] * inv;
+        t[j] = p + kMagic;
+        off = fmaxf(off, fabsf(p - (t[j] - kMagic)));
     }
-    return static_cast<int>(m);
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(t[j]);
+    if (off > 0.49997f || pre != 1.0f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float p = v[j] * pre * inv;
+            b[j] = fabsf(p - rintf(p)) > 0.49997f ? quantize_exact(v[j], p, a) : static_cast<int>(rintf(p));
+        }
+    }
+    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
+// The larger magnitude; NaN when either is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.NaN.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 template <bool VEC, int NCH, bool WARP>
 __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH>& s, RowReduce<WARP>& red, const float (&v)[8 * NCH],
-                                           int8_t* q, long long ldq, float* scale) {
+                                           int8_t* q, float* scale) {
     constexpr int N = 8 * NCH;
-    // magnitudes compare as integers, and NaN above infinity above every number
-    uint32_t m = 0;
+    float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        if (s.has(i)) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    const uint32_t top = red.max(m);
+        if (s.has(i)) m = max_abs(m, v[i]);
+    // magnitudes compare as integers, and NaN above infinity above every number
+    const uint32_t top = red.max(__float_as_uint(m) & 0x7FFFFFFFu);
     const float a = __uint_as_float(top);
     // rows without a finite, non-zero magnitude hold zeros: a zero scale gives zeros, an
     // infinite or NaN one gives NaN in every product
     const bool live = top != 0 && top < 0x7F800000u;
     // 127 / a overflows for magnitudes near the smallest: those rows are scaled up first
     const float pre = a < 1e-20f ? 0x1p100f : 1.0f;
-    const float inv = live ? 127.0f / (a * pre) : 0.0f;
+    const float inv = 127.0f / (a * pre);
     if (s.tid == 0) *scale = a / 127.0f;
     if constexpr (VEC) {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            if (s.chunk(c) >= s.D) continue;
-            uint32_t u[2] = {0, 0};
-            if (live) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    u[j >> 2] |= (static_cast<uint32_t>(quantize_value(v[8 * c + j], pre, inv, a)) & 0xFFu) << (8 * (j & 3));
-            }
-            *reinterpret_cast<uint2*>(q + s.chunk(c)) = make_uint2(u[0], u[1]);
-        }
+        for (int c = 0; c < NCH; ++c)
+            if (s.chunk(c) < s.D)
+                *reinterpret_cast<uint2*>(q + s.chunk(c)) = live ? quantize8(v + 8 * c, pre, inv, a) : make_uint2(0, 0);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (s.has(i)) q[s.elem(i)] = live ? static_cast<int8_t>(quantize_value(v[i], pre, inv, a)) : int8_t(0);
+        for (int c = 0; c < NCH; ++c) {
+            const uint2 u = live ? quantize8(v + 8 * c, pre, inv, a) : make_uint2(0, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (s.has(8 * c + j)) q[s.elem(8 * c + j)] = static_cast<int8_t>((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
+        }
     }
-    (void)ldq;
 }
 
-template <bool VEC, int NCH, bool WARP>
+// FULL: the whole operator; else only x quantised to 8 bits, in fewer registers (more rows in
+// flight: an SM needs about 40 KB of loads under way).
+template <bool VEC, int NCH, bool WARP, bool FULL>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __grid_constant__ RowNormParams p) {
     constexpr int N = 8 * NCH;
     __shared__ float red_buf[64];
@@ -267,6 +293,10 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
     for (long long row = blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * per) {
         float v[N];
         s.load_dt(p.x_dt, p.x, row * p.ldx, v);
+        if constexpr (!FULL) {
+            store_int8<VEC, NCH, WARP>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.out_scale + row);
+            continue;
+        }
         if (p.y != nullptr) {
             float t[N];
             s.load_dt(p.y_dt, p.y, row * p.ldy, t);
@@ -288,7 +318,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
         if (p.r != nullptr) s.store_dt(p.x_dt, p.r, row * p.ldr, v);
         if (p.norm != NORM_NONE) normalise<VEC, NCH, WARP>(s, red, v, p.norm, p.eps, p.w, p.b);
         if (p.out_dt == OP_I8)
-            store_int8<VEC, NCH, WARP>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.ldo, p.out_scale + row);
+            store_int8<VEC, NCH, WARP>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.out_scale + row);
         else
             s.store_dt(p.out_dt, p.out, row * p.ldo, v);
     }
@@ -299,7 +329,11 @@ void launch(cudaStream_t s, const RowNormParams& p, int threads) {
     const long long per = WARP ? threads / 32 : 1;
     long long grid = (p.rows + per - 1) / per;
     if (grid > 148 * 64) grid = 148 * 64;
-    row_norm_kernel<VEC, NCH, WARP><<<static_cast<int>(grid), threads, 0, s>>>(p);
+    const bool full = p.y != nullptr || p.r != nullptr || p.norm != NORM_NONE || p.out_dt != OP_I8 || p.alpha != 1.0f;
+    if (full)
+        row_norm_kernel<VEC, NCH, WARP, true><<<static_cast<int>(grid), threads, 0, s>>>(p);
+    else
+        row_norm_kernel<VEC, NCH, WARP, false><<<static_cast<int>(grid), threads, 0, s>>>(p);
     M3R_CUDA(cudaGetLastError());
 }
 
