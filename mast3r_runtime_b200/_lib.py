@@ -105,12 +105,12 @@ SIGNATURES = {
     "m3r_match_nn_static": (_I, [_I, _P, _P, _I64, _I64, _I, _P, _P, _P, _P]),
     "m3r_set_wait_timeout": (_I, [_P, ctypes.c_ulonglong]),
     "m3r_wait_selftest": (_I, [_I, ctypes.c_ulonglong, ctypes.POINTER(_I)]),
-    # the argument structs of the operators travel as packed bytes (ops.py)
-    "m3r_quantize_rows": (_I, [ctypes.c_char_p]),
-    "m3r_int8_linear": (_I, [ctypes.c_char_p]),
+    # operators on device buffers: pointers to their argument structs (ops.py calls them compiled)
+    "m3r_quantize_rows": (_I, [_P]),
+    "m3r_int8_linear": (_I, [_P]),
     "m3r_int8_linear_workspace": (_I64, [_I, _I64, _I64, _I64]),
-    "m3r_residual_norm": (_I, [ctypes.c_char_p]),
-    "m3r_rope": (_I, [ctypes.c_char_p]),
+    "m3r_residual_norm": (_I, [_P]),
+    "m3r_rope": (_I, [_P]),
     "m3r_operator_status": (_I, [_I, _P]),
     "m3r_check_checkpoint": (_I, [ctypes.POINTER(M3RConfig), ctypes.c_char_p]),
 }

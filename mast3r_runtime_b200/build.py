@@ -1,18 +1,22 @@
-"""Build libm3r_cuda.so (sm_100a) in-tree with nvcc.
+"""Build libm3r_cuda.so (sm_100a) in-tree with nvcc, and the torch side of ops.py with g++.
 
     python -m mast3r_runtime_b200.build          # or: python mast3r_runtime_b200/build.py
 
 Objects go to mast3r_runtime_b200/_build/ (rebuilt when a source or header is newer);
-the shared library is written next to this file so that it travels with the tree.
+the shared libraries are written next to this file so that they travel with the tree.
+_torch_ops.so (binding/torch_ops.cpp, the tensors of mast3r_runtime_b200.ops) is built against the
+torch of this interpreter, and left out where there is none: nothing else in the package needs it.
 """
 
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -20,6 +24,8 @@ CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "libm3r_cuda.so"
 INCLUDE = HERE.parent / "include"
+BINDING = HERE / "binding" / "torch_ops.cpp"
+TORCH_LIB = HERE / "_torch_ops.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -70,7 +76,37 @@ def build(verbose: bool = False) -> Path:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     if verbose:
         print(f"built {LIB}")
+    binding = build_torch_ops()
+    if verbose:
+        print(f"built {binding}" if binding else "no torch: mast3r_runtime_b200.ops is not built")
     return LIB
+
+
+def build_torch_ops() -> Path | None:
+    """_torch_ops.so, rebuilt when its source, the C header or torch's version changed."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    root = Path(spec.origin).parent
+    version = (root / "version.py").read_text()
+    stamp = BUILD / "torch_ops.version"
+    newest = max(BINDING.stat().st_mtime, (INCLUDE / "m3r_cuda.h").stat().st_mtime)
+    if TORCH_LIB.exists() and TORCH_LIB.stat().st_mtime >= newest and (
+            not stamp.exists() or stamp.read_text() == version):
+        return TORCH_LIB
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    tmp = BUILD / TORCH_LIB.name
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda),
+           str(BINDING), "-o", str(tmp), "-L", str(HERE), f"-l:{LIB.name}", "-L", str(root / "lib"),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {BINDING.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
+    stamp.write_text(version)
+    return TORCH_LIB
 
 
 if __name__ == "__main__":

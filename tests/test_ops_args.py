@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import subprocess
 import textwrap
+from struct import Struct, calcsize
 
 import pytest
 
@@ -13,9 +14,14 @@ from conftest import ROOT
 torch = pytest.importorskip("torch")
 
 
-def test_argument_structs_match_c(tmp_path):
-    from mast3r_runtime_b200 import ops
+# the argument structs of include/m3r_cuda.h, native layout
+QUANTIZE = Struct("@2i4q4P")
+LINEAR = Struct("@4i6q7PqP")
+RESIDUAL = Struct("@6i2f8q11P")
+ROPE = Struct("@5if7q2P" "2P7q" "2P7q" "P")
 
+
+def test_argument_structs_match_c(tmp_path):
     src = tmp_path / "layout.c"
     src.write_text(textwrap.dedent("""
         #include <stddef.h>
@@ -33,10 +39,8 @@ def test_argument_structs_match_c(tmp_path):
     exe = tmp_path / "layout"
     subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
     c = list(map(int, subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()))
-    from struct import calcsize
-
-    assert c == [ops._QUANTIZE.size, calcsize("@2i4q2P"), ops._LINEAR.size, calcsize("@4i6q7P"),
-                 ops._RESIDUAL.size, calcsize("@6i2f8q"), ops._ROPE.size, calcsize("@5if7q2P")]
+    assert c == [QUANTIZE.size, calcsize("@2i4q2P"), LINEAR.size, calcsize("@4i6q7P"),
+                 RESIDUAL.size, calcsize("@6i2f8q"), ROPE.size, calcsize("@5if7q2P")]
 
 
 def refused(fn, args, text):
@@ -49,10 +53,9 @@ def refused(fn, args, text):
 
 def test_c_refusals():
     """Addresses are never dereferenced: every check comes before the first CUDA call."""
-    from mast3r_runtime_b200 import ops
 
     def quantize(dev=0, dt=0, rows=2, cols=8, ldx=8, ldq=16, x=16, q=16, s=16):
-        return ops._QUANTIZE.pack(dev, dt, rows, cols, ldx, ldq, x, q, s, 0)
+        return QUANTIZE.pack(dev, dt, rows, cols, ldx, ldq, x, q, s, 0)
 
     for bad, text in ((dict(dt=3), "must be"), (dict(rows=-1), "rows out of range"), (dict(cols=0), "row length"),
                       (dict(cols=16385, ldx=16385, ldq=16400), "row length"), (dict(ldx=7), "stride"),
@@ -63,7 +66,7 @@ def test_c_refusals():
 
     def linear(xt=1, ot=1, act=0, m=4, n=32, k=64, ldx=64, ldw=64, ldo=32, x=256, xs=0, w=256, ws=256, b=0, o=256,
                work=256, size=1 << 20):
-        return ops._LINEAR.pack(0, xt, ot, act, m, n, k, ldx, ldw, ldo, x, xs, w, ws, b, o, work, size, 0)
+        return LINEAR.pack(0, xt, ot, act, m, n, k, ldx, ldw, ldo, x, xs, w, ws, b, o, work, size, 0)
 
     for bad, text in ((dict(xt=4), "x must be"), (dict(ot=3), "output must be"), (dict(act=3), "activation"),
                       (dict(m=-1), "rows out of range"), (dict(n=0), "n out of range"), (dict(k=0), "k out of range"),
@@ -77,7 +80,7 @@ def test_c_refusals():
 
     def norm(xt=2, yt=0, ot=0, kind=1, post=0, eps=1e-6, alpha=1.0, rows=4, cols=8, ldx=8, ldy=8, ldr=8, ldo=8, per=0,
              ldg=0, x=16, y=16, g=0, pw=0, pb=0, w=16, b=16, r=32, o=16, s=0):
-        return ops._RESIDUAL.pack(0, xt, yt, ot, kind, post, eps, alpha, rows, cols, ldx, ldy, ldr, ldo, per, ldg, x, y,
+        return RESIDUAL.pack(0, xt, yt, ot, kind, post, eps, alpha, rows, cols, ldx, ldy, ldr, ldo, per, ldg, x, y,
                                   g, pw, pb, w, b, r, o, s, 0)
 
     for bad, text in ((dict(xt=3), "x must be"), (dict(yt=3), "y must be"), (dict(ot=4), "output must be"),
@@ -90,7 +93,7 @@ def test_c_refusals():
         refused("m3r_residual_norm", norm(**bad), text)
 
     def rope(dt=0, axes=1, bits=64, b=1, t=4, d=64, n=32, pos=16, f=16, x=16, o=16, h=2, xt=128, ot=128):
-        return ops._ROPE.pack(0, dt, 0, axes, bits, 1.0, b, t, d, n, 0, 0, 1, pos, f, x, o, h, 0, xt, 64, 0, ot, 64,
+        return ROPE.pack(0, dt, 0, axes, bits, 1.0, b, t, d, n, 0, 0, 1, pos, f, x, o, h, 0, xt, 64, 0, ot, 64,
                               *(0,) * 9, 0)
 
     for bad, text in ((dict(dt=3), "values must be"), (dict(axes=3), "axes"), (dict(bits=16), "positions"),
