@@ -8,8 +8,10 @@
 // backends/python/rope2d.py:133-146).
 //
 // The work is bound by HBM (each value in and out once).  A block takes a few tokens: it
-// computes their sines and cosines once, in shared memory, and applies them to a range of
-// heads with 16-byte accesses.  Angles are reduced in 64 bits -- position * (inv_freq / 2 pi)
+// computes their sines and cosines once, in shared memory, while the first values are on
+// their way, and applies them to a range of heads with 16-byte accesses.  Few registers and
+// many resident blocks hide the latency (2 or 4 accesses of a thread under way at once: 140
+// and 194 us instead of 130).  Angles are reduced in 64 bits -- position * (inv_freq / 2 pi)
 // minus its nearest integer -- so that a far position keeps its fraction of a turn: in 32
 // bits position 1e6 would leave it with 2^-5 of a radian.
 #include "common.cuh"
@@ -22,9 +24,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxAngles = 2048;  // sines and cosines of a block: 16 KB
+constexpr int kMaxTokens = 32;    // tokens of a block
 
 struct RopeGrid {
     int tokens_per_block, heads_per_block, head_blocks, head_chunks;
+    int cols;  // threads along a head's chunks; kThreads / cols heads at a time
 };
 
 // VE values of T, at 2 to 16 bytes an access.
@@ -56,74 +60,99 @@ __device__ __forceinline__ T put_f(float x) {
 template <class T, int VE, bool ADJ>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p,
                                                         const __grid_constant__ RopeGrid g) {
-    __shared__ float2 turn[kMaxAngles];  // [token][frequency]: amplitude * (cos, sin)
-    const long long all = p.batch * p.tokens;
-    const long long tok0 = static_cast<long long>(blockIdx.x / g.head_blocks) * g.tokens_per_block;
+    using V = Pack<T, VE>;
+    constexpr int PAIRS = ADJ ? (VE > 1 ? VE / 2 : 1) : VE;  // pairs a chunk
+    __shared__ float2 turn[kMaxAngles];                      // [token][frequency]: amplitude * (cos, sin)
+    __shared__ double place[kMaxTokens][2];                  // the token's position on each axis
+    __shared__ long long base[kMaxTokens][4];                // its offsets in the inputs and outputs of both tensors
+    const int all = static_cast<int>(p.batch * p.tokens);
+    const int tok0 = static_cast<int>(blockIdx.x / g.head_blocks) * g.tokens_per_block;
     const int head0 = static_cast<int>(blockIdx.x % g.head_blocks) * g.heads_per_block;
-    const int heads_all = p.t[0].heads + p.t[1].heads;
-    const int heads = min(g.heads_per_block, heads_all - head0);
-    const int ntok = static_cast<int>(min(static_cast<long long>(g.tokens_per_block), all - tok0));
-    for (int i = threadIdx.x; i < ntok * p.n_freq; i += kThreads) {
-        const int tk = i / p.n_freq, f = i - tk * p.n_freq;
-        const long long tok = tok0 + tk, b = tok / p.tokens, t = tok - b * p.tokens;
-        const int axis = p.axes == 2 && f >= p.n_freq / 2;
-        const long long at = axis * p.pos_axis + b * p.pos_b + t * p.pos_t;
-        const double pos = p.pos64 ? static_cast<double>(static_cast<const long long*>(p.pos)[at])
-                                   : static_cast<double>(static_cast<const int*>(p.pos)[at]);
-        const double turns = pos * (p.inv_freq[f] * 0.15915494309189535);  // 1 / (2 pi)
-        float s, c;
-        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-        turn[i] = make_float2(c * p.amplitude, s * p.amplitude);
+    const int heads = min(g.heads_per_block, p.t[0].heads + p.t[1].heads - head0);
+    const int ntok = min(g.tokens_per_block, all - tok0);
+    const int tid = threadIdx.x;
+    if (tid < 2 * ntok) {
+        const int tk = tid >> 1, axis = tid & 1;
+        const int b = (tok0 + tk) / static_cast<int>(p.tokens), t = tok0 + tk - b * static_cast<int>(p.tokens);
+        base[tk][axis] = b * p.t[axis].xb + t * p.t[axis].xt;
+        base[tk][2 + axis] = b * p.t[axis].ob + t * p.t[axis].ot;
+        if (axis < p.axes) {
+            const long long at = axis * p.pos_axis + b * p.pos_b + t * p.pos_t;
+            place[tk][axis] = p.pos64 ? static_cast<double>(static_cast<const long long*>(p.pos)[at])
+                                      : static_cast<double>(static_cast<const int*>(p.pos)[at]);
+        }
     }
     __syncthreads();
-    constexpr int PAIRS = ADJ ? (VE > 1 ? VE / 2 : 1) : VE;  // pairs a chunk
+    // a thread's work: chunk c of (token, head) pair j, then of pair j + rows, ...
+    const int rows = kThreads / g.cols;
     const int rot_chunks = p.n_freq / PAIRS;
-    const int per_tok = heads * g.head_chunks;
-    for (int i = threadIdx.x; i < ntok * per_tok; i += kThreads) {
-        const int tk = i / per_tok;
-        const int rem = i - tk * per_tok;
-        const int hh = rem / g.head_chunks, c = rem - hh * g.head_chunks;
-        const long long tok = tok0 + tk, b = tok / p.tokens, t = tok - b * p.tokens;
-        int h = head0 + hh;
-        const RopeTensor& x = h < p.t[0].heads ? p.t[0] : p.t[1];
-        if (h >= p.t[0].heads) h -= p.t[0].heads;
-        const T* src = static_cast<const T*>(x.x) + b * x.xb + t * x.xt + h * x.xh;
-        T* dst = static_cast<T*>(x.out) + b * x.ob + t * x.ot + h * x.oh;
-        using V = Pack<T, VE>;
-        if (c >= rot_chunks) {  // behind the front part
-            const int e = 2 * p.n_freq + (c - rot_chunks) * VE;
-            *reinterpret_cast<V*>(dst + e) = *reinterpret_cast<const V*>(src + e);
-            continue;
-        }
-        const float2* w = turn + tk * p.n_freq + c * PAIRS;
-        if constexpr (!ADJ) {
-            V lo = *reinterpret_cast<const V*>(src + c * VE);
-            V hi = *reinterpret_cast<const V*>(src + p.n_freq + c * VE);
+    const int first = tid / g.cols;
+    const int pairs = first < rows ? ntok * heads : 0;
+    int c = tid % g.cols, j = first, tk = first / heads, h = first - tk * heads;
+    bool tail, two;  // behind the front part; a pair split over two accesses
+    int e0, e1;
+    T* dst;
+    V lo, hi;
+    auto load = [&]() {
+        const int second = h + head0 >= p.t[0].heads;
+        const RopeTensor& x = p.t[second];
+        const long long hh = h + head0 - (second ? p.t[0].heads : 0);
+        const T* src = static_cast<const T*>(x.x) + base[tk][second] + hh * x.xh;
+        dst = static_cast<T*>(x.out) + base[tk][2 + second] + hh * x.oh;
+        tail = c >= rot_chunks;
+        two = !tail && (!ADJ || VE == 1);
+        e0 = tail ? 2 * p.n_freq + (c - rot_chunks) * VE : ADJ && VE == 1 ? 2 * c : c * VE;
+        e1 = ADJ ? e0 + 1 : p.n_freq + c * VE;
+        lo = *reinterpret_cast<const V*>(src + e0);
+        if (two) hi = *reinterpret_cast<const V*>(src + e1);
+    };
+    bool live = j < pairs;
+    if (live) load();  // travels while the sines are computed
+    for (int i = tid; i < ntok * p.n_freq; i += kThreads) {
+        const int k = i / p.n_freq, f = i - k * p.n_freq;
+        const double turns = place[k][p.axes == 2 && f >= p.n_freq / 2] * (p.inv_freq[f] * 0.15915494309189535);  // 1 / (2 pi)
+        float sn, cs;
+        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+        turn[i] = make_float2(cs * p.amplitude, sn * p.amplitude);
+    }
+    __syncthreads();
+    while (live) {
+        if (!tail) {
+            const float2* w = turn + tk * p.n_freq + c * PAIRS;
+            if constexpr (!ADJ || VE == 1) {
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-                const float u = get_f(lo.v[j]), v = get_f(hi.v[j]);
-                const float2 a = w[j];
-                lo.v[j] = put_f<T>(u * a.x - v * a.y);
-                hi.v[j] = put_f<T>(u * a.y + v * a.x);
-            }
-            *reinterpret_cast<V*>(dst + c * VE) = lo;
-            *reinterpret_cast<V*>(dst + p.n_freq + c * VE) = hi;
-        } else if constexpr (VE > 1) {
-            V q = *reinterpret_cast<const V*>(src + c * VE);
+                for (int i = 0; i < VE; ++i) {
+                    const float a = get_f(lo.v[i]), b = get_f(hi.v[i]);
+                    const float2 r = w[i];
+                    lo.v[i] = put_f<T>(a * r.x - b * r.y);
+                    hi.v[i] = put_f<T>(a * r.y + b * r.x);
+                }
+            } else {
 #pragma unroll
-            for (int j = 0; j < VE / 2; ++j) {
-                const float u = get_f(q.v[2 * j]), v = get_f(q.v[2 * j + 1]);
-                const float2 a = w[j];
-                q.v[2 * j] = put_f<T>(u * a.x - v * a.y);
-                q.v[2 * j + 1] = put_f<T>(u * a.y + v * a.x);
+                for (int i = 0; i < VE / 2; ++i) {
+                    const float a = get_f(lo.v[2 * i]), b = get_f(lo.v[2 * i + 1]);
+                    const float2 r = w[i];
+                    lo.v[2 * i] = put_f<T>(a * r.x - b * r.y);
+                    lo.v[2 * i + 1] = put_f<T>(a * r.y + b * r.x);
+                }
             }
-            *reinterpret_cast<V*>(dst + c * VE) = q;
-        } else {
-            const float u = get_f(src[2 * c]), v = get_f(src[2 * c + 1]);
-            const float2 a = w[0];
-            dst[2 * c] = put_f<T>(u * a.x - v * a.y);
-            dst[2 * c + 1] = put_f<T>(u * a.y + v * a.x);
         }
+        *reinterpret_cast<V*>(dst + e0) = lo;
+        if (two) *reinterpret_cast<V*>(dst + e1) = hi;
+        j += rows;
+        h += rows;
+        while (h >= heads) {
+            h -= heads;
+            ++tk;
+        }
+        if (j >= pairs) {  // the next chunk, of heads with more chunks than a block has threads
+            c += g.cols;
+            j = first;
+            tk = first / heads;
+            h = first - tk * heads;
+            live = c < g.head_chunks;
+        }
+        if (live) load();
     }
 }
 
@@ -134,21 +163,23 @@ void launch(cudaStream_t s, const RopeParams& p) {
     const int heads = p.t[0].heads + p.t[1].heads;
     RopeGrid g;
     g.head_chunks = p.n_freq / PAIRS + (p.dim - 2 * p.n_freq) / VE;
-    // tokens a block: enough for every thread to have a sine, heads split over blocks while
-    // there are few tokens (each block then recomputes its tokens' sines)
-    g.tokens_per_block = kMaxAngles / p.n_freq;
-    if (g.tokens_per_block > 8) g.tokens_per_block = 8;
-    while (g.tokens_per_block > 1 && all / g.tokens_per_block < 2 * 148) g.tokens_per_block /= 2;
+    g.cols = g.head_chunks < kThreads ? g.head_chunks : kThreads;
+    // tokens a block: 8 accesses for every thread (2 to 16 measured, on 98,304 tokens of 32 heads of 64:
+    // 148, 135, 130, 134 us); while there are few tokens, fewer, and then the heads split over blocks
+    // (each computes its tokens' sines)
+    const int rows = kThreads / g.cols;
+    g.tokens_per_block = rows * 8 / heads > 1 ? rows * 8 / heads : 1;
+    if (g.tokens_per_block > kMaxTokens) g.tokens_per_block = kMaxTokens;
+    if (g.tokens_per_block > kMaxAngles / p.n_freq) g.tokens_per_block = kMaxAngles / p.n_freq;
+    while (g.tokens_per_block > 1 && all / g.tokens_per_block < 4 * 148) g.tokens_per_block /= 2;
     const long long token_blocks = (all + g.tokens_per_block - 1) / g.tokens_per_block;
     g.heads_per_block = heads;
-    const long long want = 2 * 148;
+    const long long want = 4 * 148;
     if (token_blocks < want) {
-        long long split = want / token_blocks;
-        if (split > heads) split = heads;
+        const long long split = want / token_blocks < heads ? want / token_blocks : heads;
         g.heads_per_block = static_cast<int>((heads + split - 1) / split);
-        // at least one chunk for every thread
-        const int least = (kThreads + g.tokens_per_block * g.head_chunks - 1) / (g.tokens_per_block * g.head_chunks);
-        if (g.heads_per_block < least) g.heads_per_block = least < heads ? least : heads;
+        // at least one access for every thread
+        if (g.heads_per_block < rows) g.heads_per_block = rows < heads ? rows : heads;
     }
     g.head_blocks = (heads + g.heads_per_block - 1) / g.heads_per_block;
     const long long grid = token_blocks * g.head_blocks;

@@ -41,12 +41,19 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) {
 template <bool VEC, int NCH>
 struct RowSlice {
     int tid, G, D;
+    int id[VEC ? 1 : 8 * NCH];  // the elements, those behind the row's end moved to its last
+    __device__ __forceinline__ RowSlice(int tid_, int G_, int D_) : tid(tid_), G(G_), D(D_) {
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int i = 0; i < 8 * NCH; ++i) id[i] = min(elem(i), D - 1);
+        }
+    }
     __device__ __forceinline__ int chunk(int c) const { return (tid + c * G) * 8; }
     __device__ __forceinline__ int elem(int i) const { return VEC ? chunk(i >> 3) + (i & 7) : tid + i * G; }
     __device__ __forceinline__ bool has(int i) const { return (VEC ? chunk(i >> 3) : elem(i)) < D; }
 
     template <class T>
-    __device__ __forceinline__ void load(const T* p, float (&v)[8 * NCH], float fill) const {
+    __device__ __forceinline__ void load(const T* p, float (&v)[8 * NCH]) const {
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
@@ -68,21 +75,44 @@ struct RowSlice {
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[8 * c + j] = fill;
+                    for (int j = 0; j < 8; ++j) v[8 * c + j] = 0.0f;
                 }
             }
         } else {
+            // no condition around the loads: a branch around each would wait for them one by one
+            T t[8 * NCH];
 #pragma unroll
-            for (int i = 0; i < 8 * NCH; ++i) v[i] = elem(i) < D ? to_f(p[elem(i)]) : fill;
+            for (int i = 0; i < 8 * NCH; ++i) t[i] = p[id[i]];
+#pragma unroll
+            for (int i = 0; i < 8 * NCH; ++i) v[i] = has(i) ? to_f(t[i]) : 0.0f;
+        }
+    }
+    // Values 8 c .. 8 c + 8 of a float vector as long as the row (zero behind its end), or `none`
+    // where there is no vector.
+    __device__ __forceinline__ void vector8(const float* p, int c, float none, float (&o)[8]) const {
+        if (p == nullptr) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = none;
+        } else if constexpr (VEC) {
+            const float4* q = reinterpret_cast<const float4*>(p + min(chunk(c), D - 8));
+            const float4 a = __ldg(q), b = __ldg(q + 1);
+            const bool in = chunk(c) < D;
+            o[0] = in ? a.x : 0.0f, o[1] = in ? a.y : 0.0f, o[2] = in ? a.z : 0.0f, o[3] = in ? a.w : 0.0f;
+            o[4] = in ? b.x : 0.0f, o[5] = in ? b.y : 0.0f, o[6] = in ? b.z : 0.0f, o[7] = in ? b.w : 0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = __ldg(p + id[8 * c + j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = has(8 * c + j) ? o[j] : 0.0f;
         }
     }
     __device__ __forceinline__ void load_dt(int dt, const void* base, long long off, float (&v)[8 * NCH]) const {
         if (dt == OP_F32)
-            load(static_cast<const float*>(base) + off, v, 0.0f);
+            load(static_cast<const float*>(base) + off, v);
         else if (dt == OP_F16)
-            load(static_cast<const __half*>(base) + off, v, 0.0f);
+            load(static_cast<const __half*>(base) + off, v);
         else
-            load(static_cast<const __nv_bfloat16*>(base) + off, v, 0.0f);
+            load(static_cast<const __nv_bfloat16*>(base) + off, v);
     }
     template <class T>
     __device__ __forceinline__ void store(T* p, const float (&v)[8 * NCH]) const {
@@ -179,25 +209,13 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH>& s, RowReduce
     }
     const float rstd = rsqrtf(red.sum(q) * inv_d + eps);
     // the weight and bias vectors are read chunk by chunk: every row reads them from L1
-    if constexpr (VEC) {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            if (s.chunk(c) >= s.D) continue;
+    for (int c = 0; c < NCH; ++c) {
+        float g[8], a[8];
+        s.vector8(w, c, 1.0f, g);
+        s.vector8(b, c, 0.0f, a);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float* u = v + 8 * c + 4 * h;
-                const float4 g = w ? __ldg(reinterpret_cast<const float4*>(w + s.chunk(c)) + h) : make_float4(1, 1, 1, 1);
-                const float4 a = b ? __ldg(reinterpret_cast<const float4*>(b + s.chunk(c)) + h) : make_float4(0, 0, 0, 0);
-                u[0] = u[0] * rstd * g.x + a.x;
-                u[1] = u[1] * rstd * g.y + a.y;
-                u[2] = u[2] * rstd * g.z + a.z;
-                u[3] = u[3] * rstd * g.w + a.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (s.has(i)) v[i] = v[i] * rstd * (w ? __ldg(w + s.elem(i)) : 1.0f) + (b ? __ldg(b + s.elem(i)) : 0.0f);
+        for (int j = 0; j < 8; ++j) v[8 * c + j] = v[8 * c + j] * rstd * g[j] + a[j];
     }
 }
 
@@ -210,27 +228,50 @@ __device__ __noinline__ int quantize_exact(float v, float p, float a) {
     return d > 0.0 ? l + 1 : d < 0.0 ? l : (l & 1) ? l + 1 : l;
 }
 
-// Eight values in 8 bits.  p = v * inv lies within 2e-5 of 127 v / a (two roundings of a value up
-// to 127), so that its nearest integer is the right one unless p is that near to a half: one test
-// for the eight, taken for about one value in 10^5, sends them to quantize_exact.  Adding 1.5 * 2^23
-// rounds p to the integer that then stands in the sum's low byte.
-__device__ __forceinline__ uint2 quantize8(const float* v, float pre, float inv, float a) {
-    constexpr float kMagic = 12582912.0f;
-    float t[8], off = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float p = v[j] * inv;
-        t[j] = p + kMagic;
-        off = fmaxf(off, fabsf(p - (t[j] - kMagic)));
+// A row's scaling to 8 bits.  The row is first scaled by a power of two that keeps 127 v and 1 / a
+// away from the ends of the 32-bit range; k = 127 times that power.
+struct Quantizer {
+    float a, top, k, inv;  // largest magnitude, the same scaled, 127 scaled, 1 / top
+    __device__ __forceinline__ explicit Quantizer(float largest) : a(largest) {
+        const float pre = a < 0x1p-60f ? 0x1p90f : a > 0x1p60f ? 0x1p-60f : 1.0f;
+        top = a * pre;
+        k = 127.0f * pre;
+        inv = 1.0f / top;
     }
+    // The quotient t / top for t = k v: for 16-bit v, t, the remainder and a quotient halfway between
+    // two levels are exact in 32 bits, and any other quotient is 2^-19 away from half a level, so that
+    // one correction makes its nearest integer the right one.
+    __device__ __forceinline__ float quotient16(float v) const {
+        const float t = v * k, q = t * inv;
+        return fmaf(fmaf(-q, top, t), inv, q);
+    }
+};
+
+// Eight values in 8 bits: adding 1.5 * 2^23 rounds the quotient to the integer that then stands in
+// the sum's low byte.  32-bit values: k v * inv lies within 3e-5 of 127 v / a (three roundings of a
+// value up to 127), which decides unless it is that near to a half; one test for the eight, taken
+// for about one value in 10^4, sends them to quantize_exact.
+template <bool EXACT16>
+__device__ __forceinline__ uint2 quantize8(const float* v, const Quantizer& z) {
+    constexpr float kMagic = 12582912.0f;
     uint32_t b[8];
+    if constexpr (EXACT16) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(t[j]);
-    if (off > 0.49997f || pre != 1.0f) {
+        for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(z.quotient16(v[j]) + kMagic);
+    } else {
+        float off = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float p = v[j] * pre * inv;
-            b[j] = fabsf(p - rintf(p)) > 0.49997f ? quantize_exact(v[j], p, a) : static_cast<int>(rintf(p));
+            const float p = v[j] * z.k * z.inv, t = p + kMagic;
+            off = fmaxf(off, fabsf(p - (t - kMagic)));
+            b[j] = __float_as_uint(t);
+        }
+        if (off > 0.49996f) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float p = v[j] * z.k * z.inv;
+                if (fabsf(p - rintf(p)) > 0.49996f) b[j] = quantize_exact(v[j], p, z.a);
+            }
         }
     }
     return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
@@ -244,33 +285,27 @@ __device__ __forceinline__ float max_abs(float a, float b) {
     return r;
 }
 
-template <bool VEC, int NCH, bool WARP>
+template <bool EXACT16, bool VEC, int NCH, bool WARP>
 __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH>& s, RowReduce<WARP>& red, const float (&v)[8 * NCH],
                                            int8_t* q, float* scale) {
     constexpr int N = 8 * NCH;
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (s.has(i)) m = max_abs(m, v[i]);
+    for (int i = 0; i < N; ++i) m = max_abs(m, s.has(i) ? v[i] : 0.0f);
     // magnitudes compare as integers, and NaN above infinity above every number
     const uint32_t top = red.max(__float_as_uint(m) & 0x7FFFFFFFu);
-    const float a = __uint_as_float(top);
     // rows without a finite, non-zero magnitude hold zeros: a zero scale gives zeros, an
     // infinite or NaN one gives NaN in every product
     const bool live = top != 0 && top < 0x7F800000u;
-    // 127 / a overflows for magnitudes near the smallest: those rows are scaled up first
-    const float pre = a < 1e-20f ? 0x1p100f : 1.0f;
-    const float inv = 127.0f / (a * pre);
-    if (s.tid == 0) *scale = a / 127.0f;
-    if constexpr (VEC) {
+    const Quantizer z(__uint_as_float(top));
+    if (s.tid == 0) *scale = z.a / 127.0f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c)
-            if (s.chunk(c) < s.D)
-                *reinterpret_cast<uint2*>(q + s.chunk(c)) = live ? quantize8(v + 8 * c, pre, inv, a) : make_uint2(0, 0);
-    } else {
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const uint2 u = live ? quantize8(v + 8 * c, pre, inv, a) : make_uint2(0, 0);
+    for (int c = 0; c < NCH; ++c) {
+        if (VEC && s.chunk(c) >= s.D) continue;
+        const uint2 u = live ? quantize8<EXACT16>(v + 8 * c, z) : make_uint2(0, 0);
+        if constexpr (VEC) {
+            *reinterpret_cast<uint2*>(q + s.chunk(c)) = u;
+        } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (s.has(8 * c + j)) q[s.elem(8 * c + j)] = static_cast<int8_t>((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
@@ -278,23 +313,24 @@ __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH>& s, RowReduc
     }
 }
 
-// FULL: the whole operator; else only x quantised to 8 bits, in fewer registers (more rows in
-// flight: an SM needs about 40 KB of loads under way).
-template <bool VEC, int NCH, bool WARP, bool FULL>
+// What a kernel does: the whole operator, or only x quantised to 8 bits, in fewer registers (more
+// rows in flight: an SM needs about 40 KB of loads under way).
+enum RowMode : int { ROW_FULL = 0, ROW_QUANTIZE_F32 = 1, ROW_QUANTIZE_16 = 2 };
+
+template <bool VEC, int NCH, bool WARP, int MODE>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __grid_constant__ RowNormParams p) {
     constexpr int N = 8 * NCH;
     __shared__ float red_buf[64];
     RowReduce<WARP> red{red_buf, 0};
-    RowSlice<VEC, NCH> s;
-    s.D = p.cols;
-    s.G = WARP ? 32 : static_cast<int>(blockDim.x);
-    s.tid = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
+    const RowSlice<VEC, NCH> s(WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
+                               WARP ? 32 : static_cast<int>(blockDim.x), p.cols);
     const long long per = WARP ? blockDim.x >> 5 : 1;
     for (long long row = blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * per) {
         float v[N];
         s.load_dt(p.x_dt, p.x, row * p.ldx, v);
-        if constexpr (!FULL) {
-            store_int8<VEC, NCH, WARP>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.out_scale + row);
+        if constexpr (MODE != ROW_FULL) {
+            store_int8<MODE == ROW_QUANTIZE_16>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo,
+                                                p.out_scale + row);
             continue;
         }
         if (p.y != nullptr) {
@@ -303,10 +339,13 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
             if (p.post != NORM_NONE) normalise<VEC, NCH, WARP>(s, red, t, p.post, p.eps, p.pw, p.pb);
             if (p.gate != nullptr) {
                 const float* g = p.gate + (row / p.rows_per_gate) * p.ld_gate;
-                float gv[N];
-                s.load(g, gv, 0.0f);
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = p.alpha * v[i] + gv[i] * t[i];
+                for (int c = 0; c < NCH; ++c) {
+                    float gv[8];
+                    s.vector8(g, c, 1.0f, gv);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[8 * c + j] = p.alpha * v[8 * c + j] + gv[j] * t[8 * c + j];
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[i] = p.alpha * v[i] + t[i];
@@ -318,7 +357,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
         if (p.r != nullptr) s.store_dt(p.x_dt, p.r, row * p.ldr, v);
         if (p.norm != NORM_NONE) normalise<VEC, NCH, WARP>(s, red, v, p.norm, p.eps, p.w, p.b);
         if (p.out_dt == OP_I8)
-            store_int8<VEC, NCH, WARP>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.out_scale + row);
+            store_int8<false>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.out_scale + row);
         else
             s.store_dt(p.out_dt, p.out, row * p.ldo, v);
     }
@@ -331,9 +370,11 @@ void launch(cudaStream_t s, const RowNormParams& p, int threads) {
     if (grid > 148 * 64) grid = 148 * 64;
     const bool full = p.y != nullptr || p.r != nullptr || p.norm != NORM_NONE || p.out_dt != OP_I8 || p.alpha != 1.0f;
     if (full)
-        row_norm_kernel<VEC, NCH, WARP, true><<<static_cast<int>(grid), threads, 0, s>>>(p);
+        row_norm_kernel<VEC, NCH, WARP, ROW_FULL><<<static_cast<int>(grid), threads, 0, s>>>(p);
+    else if (p.x_dt == OP_F32)
+        row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_F32><<<static_cast<int>(grid), threads, 0, s>>>(p);
     else
-        row_norm_kernel<VEC, NCH, WARP, false><<<static_cast<int>(grid), threads, 0, s>>>(p);
+        row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_16><<<static_cast<int>(grid), threads, 0, s>>>(p);
     M3R_CUDA(cudaGetLastError());
 }
 
@@ -341,13 +382,21 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * op_size(dt)) % bytes == 0);
 }
 
+// Rows to warps or blocks.  With many rows, a warp each up to 1,024 values (98,304 rows of 1,024,
+// 32-bit stream: 211 us, against 226 with a block each); with few, and for element accesses, a
+// block each, 8 values a thread, so that a row's chain of loads and reductions is short (1,536 rows
+// of 1,024 quantised: 4.0 us against 6.8).
 template <bool VEC>
 void dispatch(cudaStream_t s, const RowNormParams& p) {
     if (p.cols <= 256) return launch<VEC, 1, true>(s, p, 128);
-    if (p.cols <= 512) return launch<VEC, 2, true>(s, p, 128);
-    if (p.cols <= 1024) return launch<VEC, 4, true>(s, p, 128);
+    if constexpr (VEC) {
+        if (p.rows > 148 * 16) {
+            if (p.cols <= 512) return launch<VEC, 2, true>(s, p, 128);
+            if (p.cols <= 1024) return launch<VEC, 4, true>(s, p, 128);
+        }
+    }
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
-    if (p.cols <= 8192 && p.rows < 2 * 148) return launch<VEC, 1, false>(s, p, threads(1));
+    if (p.cols <= 1024 || (p.cols <= 8192 && (!VEC || p.rows <= 148 * 2))) return launch<VEC, 1, false>(s, p, threads(1));
     launch<VEC, 2, false>(s, p, threads(2));
 }
 

@@ -79,6 +79,28 @@ def test_quantize_ties_and_tiny_magnitudes(ops):
     assert int(q[4].abs().max()) == 0 and float(s[4]) == 0 and int(q[5, 3]) == 127
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_quantize_every_16_bit_value(ops, dtype):
+    """Every finite value of the type up to a row's largest one, for largest ones with many ties
+    (127 and 1 times powers of two), few, and at both ends of the type's range."""
+    t = DT[dtype]
+    bits = torch.arange(0, 2 ** 15, dtype=torch.int32).to(torch.int16).view(t)
+    bits = bits[torch.isfinite(bits)]
+    fi = torch.finfo(t)
+    for a in (1.0, 127.0, 254.0, 3.0, 1.9, 0.01, fi.max, fi.tiny, fi.smallest_normal / 2 ** 5, 2.0 ** 15 * 1.25):
+        a = torch.tensor(a).to(t)
+        v = bits[(bits <= a) & (bits >= a.float() / 4096)]
+        v = torch.cat([v, -v, a[None]])
+        x = torch.zeros(-(-v.numel() // 4000), 4001, dtype=t)
+        x[:, 0] = a  # the largest one in every row
+        for i in range(x.shape[0]):
+            part = v[i * 4000:(i + 1) * 4000]
+            x[i, 1:1 + part.numel()] = part
+        x = x.cuda()
+        q, s = ops.quantize_rows(x)
+        assert torch.equal(q, levels(x)[0]), float(a)
+
+
 def test_quantize_non_finite_rows_and_strides(ops):
     base = rnd(6, 40, 96, seed=3, dtype=torch.bfloat16)
     x = base[:, ::2, 8:83]  # rows evenly spaced within a block of 20, not across blocks
