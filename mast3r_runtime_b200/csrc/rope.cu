@@ -58,7 +58,7 @@ __device__ __forceinline__ T put_f(float x) {
 // accesses each), the adjacent one 2 n_freq / VE of VE / 2 pairs; then the chunks of the tail.
 // VE = 1 of the adjacent layout takes a pair a chunk.
 template <class T, int VE, bool ADJ>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p,
+__global__ void __launch_bounds__(kThreads, 6) rope_kernel(const __grid_constant__ RopeParams p,
                                                         const __grid_constant__ RopeGrid g) {
     using V = Pack<T, VE>;
     constexpr int PAIRS = ADJ ? (VE > 1 ? VE / 2 : 1) : VE;  // pairs a chunk

@@ -37,20 +37,16 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) {
 }
 
 // The N = 8 * NCH values of a thread.  VEC: chunk c holds elements (tid + c * G) * 8 .. + 8
-// of the row (one 16-byte access of a 16-bit type); else value i is element tid + i * G.
-template <bool VEC, int NCH>
+// of the row (one 16-byte access of a 16-bit type); else value i is element tid + i * G, with G
+// (GT, the block's threads) known to the compiler, so that an access is one instruction.
+template <bool VEC, int NCH, int GT>
 struct RowSlice {
-    int tid, G, D;
-    int id[VEC ? 1 : 8 * NCH];  // the elements, those behind the row's end moved to its last
-    __device__ __forceinline__ RowSlice(int tid_, int G_, int D_) : tid(tid_), G(G_), D(D_) {
-        if constexpr (!VEC) {
-#pragma unroll
-            for (int i = 0; i < 8 * NCH; ++i) id[i] = min(elem(i), D - 1);
-        }
-    }
-    __device__ __forceinline__ int chunk(int c) const { return (tid + c * G) * 8; }
-    __device__ __forceinline__ int elem(int i) const { return VEC ? chunk(i >> 3) + (i & 7) : tid + i * G; }
-    __device__ __forceinline__ bool has(int i) const { return (VEC ? chunk(i >> 3) : elem(i)) < D; }
+    int tid, D, rem;  // rem: elements from tid on
+    int Gv;
+    __device__ __forceinline__ RowSlice(int tid_, int G_, int D_) : tid(tid_), D(D_), rem(D_ - tid_), Gv(G_) {}
+    __device__ __forceinline__ int G() const { return VEC ? Gv : GT; }
+    __device__ __forceinline__ int chunk(int c) const { return (tid + c * G()) * 8; }
+    __device__ __forceinline__ bool has(int i) const { return VEC ? chunk(i >> 3) < D : rem > i * GT; }
 
     template <class T>
     __device__ __forceinline__ void load(const T* p, float (&v)[8 * NCH]) const {
@@ -79,12 +75,9 @@ struct RowSlice {
                 }
             }
         } else {
-            // no condition around the loads: a branch around each would wait for them one by one
-            T t[8 * NCH];
+            p += tid;
 #pragma unroll
-            for (int i = 0; i < 8 * NCH; ++i) t[i] = p[id[i]];
-#pragma unroll
-            for (int i = 0; i < 8 * NCH; ++i) v[i] = has(i) ? to_f(t[i]) : 0.0f;
+            for (int i = 0; i < 8 * NCH; ++i) v[i] = has(i) ? to_f(p[i * GT]) : 0.0f;
         }
     }
     // Values 8 c .. 8 c + 8 of a float vector as long as the row (zero behind its end), or `none`
@@ -100,10 +93,9 @@ struct RowSlice {
             o[0] = in ? a.x : 0.0f, o[1] = in ? a.y : 0.0f, o[2] = in ? a.z : 0.0f, o[3] = in ? a.w : 0.0f;
             o[4] = in ? b.x : 0.0f, o[5] = in ? b.y : 0.0f, o[6] = in ? b.z : 0.0f, o[7] = in ? b.w : 0.0f;
         } else {
+            p += tid;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = __ldg(p + id[8 * c + j]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = has(8 * c + j) ? o[j] : 0.0f;
+            for (int j = 0; j < 8; ++j) o[j] = has(8 * c + j) ? __ldg(p + (8 * c + j) * GT) : 0.0f;
         }
     }
     __device__ __forceinline__ void load_dt(int dt, const void* base, long long off, float (&v)[8 * NCH]) const {
@@ -134,13 +126,14 @@ struct RowSlice {
                 }
             }
         } else {
+            p += tid;
 #pragma unroll
             for (int i = 0; i < 8 * NCH; ++i)
-                if (elem(i) < D) {
+                if (has(i)) {
                     if constexpr (sizeof(T) == 4)
-                        p[elem(i)] = v[i];
+                        p[i * GT] = v[i];
                     else
-                        p[elem(i)] = Elem<T>::from(v[i]);
+                        p[i * GT] = Elem<T>::from(v[i]);
                 }
         }
     }
@@ -189,8 +182,8 @@ struct RowReduce {
     }
 };
 
-template <bool VEC, int NCH, bool WARP>
-__device__ __forceinline__ void normalise(const RowSlice<VEC, NCH>& s, RowReduce<WARP>& red, float (&v)[8 * NCH],
+template <bool VEC, int NCH, bool WARP, int GT>
+__device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowReduce<WARP>& red, float (&v)[8 * NCH],
                                           int kind, float eps, const float* w, const float* b) {
     constexpr int N = 8 * NCH;
     const float inv_d = 1.0f / static_cast<float>(s.D);
@@ -285,8 +278,8 @@ __device__ __forceinline__ float max_abs(float a, float b) {
     return r;
 }
 
-template <bool EXACT16, bool VEC, int NCH, bool WARP>
-__device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH>& s, RowReduce<WARP>& red, const float (&v)[8 * NCH],
+template <bool EXACT16, bool VEC, int NCH, bool WARP, int GT>
+__device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH, GT>& s, RowReduce<WARP>& red, const float (&v)[8 * NCH],
                                            int8_t* q, float* scale) {
     constexpr int N = 8 * NCH;
     float m = 0.0f;
@@ -308,7 +301,7 @@ __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH>& s, RowReduc
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (s.has(8 * c + j)) q[s.elem(8 * c + j)] = static_cast<int8_t>((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
+                if (s.has(8 * c + j)) q[s.tid + (8 * c + j) * GT] = static_cast<int8_t>((j < 4 ? u.x : u.y) >> (8 * (j & 3)));
         }
     }
 }
@@ -317,13 +310,13 @@ __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH>& s, RowReduc
 // rows in flight: an SM needs about 40 KB of loads under way).
 enum RowMode : int { ROW_FULL = 0, ROW_QUANTIZE_F32 = 1, ROW_QUANTIZE_16 = 2 };
 
-template <bool VEC, int NCH, bool WARP, int MODE>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __grid_constant__ RowNormParams p) {
+template <bool VEC, int NCH, bool WARP, int MODE, int GT>
+__global__ void __launch_bounds__(WARP ? 128 : VEC ? 1024 : GT, WARP && NCH == 4 && MODE == ROW_FULL ? 5 : 0) row_norm_kernel(const __grid_constant__ RowNormParams p) {
     constexpr int N = 8 * NCH;
     __shared__ float red_buf[64];
     RowReduce<WARP> red{red_buf, 0};
-    const RowSlice<VEC, NCH> s(WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
-                               WARP ? 32 : static_cast<int>(blockDim.x), p.cols);
+    const RowSlice<VEC, NCH, GT> s(WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
+                               WARP ? 32 : VEC ? static_cast<int>(blockDim.x) : GT, p.cols);
     const long long per = WARP ? blockDim.x >> 5 : 1;
     for (long long row = blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * per) {
         float v[N];
@@ -336,9 +329,10 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
         if (p.y != nullptr) {
             float t[N];
             s.load_dt(p.y_dt, p.y, row * p.ldy, t);
-            if (p.post != NORM_NONE) normalise<VEC, NCH, WARP>(s, red, t, p.post, p.eps, p.pw, p.pb);
+            if (p.post != NORM_NONE) normalise(s, red, t, p.post, p.eps, p.pw, p.pb);
             if (p.gate != nullptr) {
-                const float* g = p.gate + (row / p.rows_per_gate) * p.ld_gate;
+                const float* g = p.gate;
+                if (p.ld_gate != 0) g += static_cast<long long>(static_cast<uint32_t>(row) / static_cast<uint32_t>(p.rows_per_gate)) * p.ld_gate;
 #pragma unroll
                 for (int c = 0; c < NCH; ++c) {
                     float gv[8];
@@ -355,7 +349,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
             for (int i = 0; i < N; ++i) v[i] *= p.alpha;
         }
         if (p.r != nullptr) s.store_dt(p.x_dt, p.r, row * p.ldr, v);
-        if (p.norm != NORM_NONE) normalise<VEC, NCH, WARP>(s, red, v, p.norm, p.eps, p.w, p.b);
+        if (p.norm != NORM_NONE) normalise(s, red, v, p.norm, p.eps, p.w, p.b);
         if (p.out_dt == OP_I8)
             store_int8<false>(s, red, v, static_cast<int8_t*>(p.out) + row * p.ldo, p.out_scale + row);
         else
@@ -363,18 +357,16 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) row_norm_kernel(const __gri
     }
 }
 
-template <bool VEC, int NCH, bool WARP>
+template <bool VEC, int NCH, bool WARP, int GT = 0>
 void launch(cudaStream_t s, const RowNormParams& p, int threads) {
     const long long per = WARP ? threads / 32 : 1;
     long long grid = (p.rows + per - 1) / per;
     if (grid > 148 * 64) grid = 148 * 64;
     const bool full = p.y != nullptr || p.r != nullptr || p.norm != NORM_NONE || p.out_dt != OP_I8 || p.alpha != 1.0f;
-    if (full)
-        row_norm_kernel<VEC, NCH, WARP, ROW_FULL><<<static_cast<int>(grid), threads, 0, s>>>(p);
-    else if (p.x_dt == OP_F32)
-        row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_F32><<<static_cast<int>(grid), threads, 0, s>>>(p);
-    else
-        row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_16><<<static_cast<int>(grid), threads, 0, s>>>(p);
+    auto kern = full                ? row_norm_kernel<VEC, NCH, WARP, ROW_FULL, GT>
+                : p.x_dt == OP_F32 ? row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_F32, GT>
+                                   : row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_16, GT>;
+    kern<<<static_cast<int>(grid), threads, 0, s>>>(p);
     M3R_CUDA(cudaGetLastError());
 }
 
@@ -383,21 +375,30 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
 }
 
 // Rows to warps or blocks.  With many rows, a warp each up to 1,024 values (98,304 rows of 1,024,
-// 32-bit stream: 211 us, against 226 with a block each); with few, and for element accesses, a
-// block each, 8 values a thread, so that a row's chain of loads and reductions is short (1,536 rows
-// of 1,024 quantised: 4.0 us against 6.8).
-template <bool VEC>
-void dispatch(cudaStream_t s, const RowNormParams& p) {
-    if (p.cols <= 256) return launch<VEC, 1, true>(s, p, 128);
-    if constexpr (VEC) {
-        if (p.rows > 148 * 16) {
-            if (p.cols <= 512) return launch<VEC, 2, true>(s, p, 128);
-            if (p.cols <= 1024) return launch<VEC, 4, true>(s, p, 128);
-        }
+// 32-bit stream: 199 us, against 226 with a block each); with few, a block each, 8 values a
+// thread, so that a row's chain of loads and reductions is short (1,536 rows of 1,024 quantised:
+// 4.0 us against 6.8).
+void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
+    if (p.cols <= 256) return launch<true, 1, true>(s, p, 128);
+    if (p.rows > 148 * 16) {
+        if (p.cols <= 512) return launch<true, 2, true>(s, p, 128);
+        if (p.cols <= 1024) return launch<true, 4, true>(s, p, 128);
     }
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
-    if (p.cols <= 1024 || (p.cols <= 8192 && (!VEC || p.rows <= 148 * 2))) return launch<VEC, 1, false>(s, p, threads(1));
-    launch<VEC, 2, false>(s, p, threads(2));
+    if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, false>(s, p, threads(1));
+    launch<true, 2, false>(s, p, threads(2));
+}
+
+// Element accesses (odd widths, rows off the 16-byte grid): 8 values a thread, neighbouring
+// threads at neighbouring elements.
+void dispatch_elements(cudaStream_t s, const RowNormParams& p) {
+    if (p.cols <= 256) return launch<false, 1, true, 32>(s, p, 128);
+    if (p.cols <= 512) return launch<false, 1, false, 64>(s, p, 64);
+    if (p.cols <= 1024) return launch<false, 1, false, 128>(s, p, 128);
+    if (p.cols <= 2048) return launch<false, 1, false, 256>(s, p, 256);
+    if (p.cols <= 4096) return launch<false, 1, false, 512>(s, p, 512);
+    if (p.cols <= 8192) return launch<false, 1, false, 1024>(s, p, 1024);
+    launch<false, 2, false, 1024>(s, p, 1024);
 }
 
 }  // namespace
@@ -410,9 +411,9 @@ void row_norm(cudaStream_t s, const RowNormParams& p) {
                      aligned(p.gate, p.ld_gate, OP_F32, 16) && aligned(p.pw, 0, OP_F32, 16) &&
                      aligned(p.pb, 0, OP_F32, 16) && aligned(p.w, 0, OP_F32, 16) && aligned(p.b, 0, OP_F32, 16);
     if (vec)
-        dispatch<true>(s, p);
+        dispatch_vec(s, p);
     else
-        dispatch<false>(s, p);
+        dispatch_elements(s, p);
 }
 
 }  // namespace m3r
