@@ -24,6 +24,16 @@ namespace {
 // First wait of any operator kernel that ran out on this device (see mbar_wait).
 __device__ DevStatus g_status;
 
+}  // namespace
+
+}  // namespace m3r
+
+#include "int8_small.cuh"
+
+namespace m3r {
+
+namespace {
+
 constexpr int kEpiWarps = 8;
 constexpr int kEpiGroups = kEpiWarps / 4;         // warps that share a TMEM lane quarter
 constexpr int kWarpCols = 256 / kEpiGroups;       // most columns of a tile that one warp handles
@@ -500,21 +510,24 @@ int sm_count(int dev) {
     return n[dev];
 }
 
-template <int BN, int CG>
-void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long long ldq, const float* xs) {
-    using C = I8Cfg<BN, CG>;
-    auto kern = int8_gemm_kernel<BN, CG>;
+// Raises a kernel's shared memory limit once on each device.
+template <class Kernel>
+void allow_smem(Kernel kern, int bytes, unsigned& done) {
     int dev = 0;
     M3R_CUDA(cudaGetDevice(&dev));
-    {
-        static std::mutex mu;
-        static unsigned done = 0;  // devices whose limit is raised
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev >= 32 || !(done >> dev & 1)) {
-            M3R_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
-            if (dev < 32) done |= 1u << dev;
-        }
-    }
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev < 32 && (done >> dev & 1)) return;
+    M3R_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 32) done |= 1u << dev;
+}
+
+template <int BN, int CG>
+void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long long ldq, const float* xs, int sms) {
+    using C = I8Cfg<BN, CG>;
+    auto kern = int8_gemm_kernel<BN, CG>;
+    static unsigned done = 0;
+    allow_smem(kern, C::SMEM_BYTES, done);
     Int8Params p;
     p.M = static_cast<int>(q.rows);
     p.N = q.n;
@@ -536,7 +549,7 @@ void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long lo
         mc = q.out_dt == OP_F32 ? tmap_2d_f32(q.out, q.rows, q.n, q.ldo, 32)
                                 : tmap_2d(q.out_dt, q.out, q.rows, q.n, q.ldo, 32);
     const int units = p.tiles_m * p.tiles_n;
-    const int max_units = sm_count(dev) / CG;
+    const int max_units = sms / CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(CG * (units < max_units ? units : max_units));
     cfg.blockDim = dim3(kThreads);
@@ -552,20 +565,95 @@ void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long lo
     M3R_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, p));
 }
 
+template <int NT>
+void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long long ldq, const float* xs, int sms) {
+    using C = SkinnyCfg<NT>;
+    auto kern = int8_skinny_kernel<NT>;
+    static unsigned done = 0;
+    allow_smem(kern, C::SMEM_BYTES, done);
+    SkinnyParams p;
+    p.M = static_cast<int>(q.rows);
+    p.N = q.n;
+    p.num_kb = cdiv(q.k, 128);
+    p.xs = xs;
+    p.ws = q.w_scale;
+    p.bias = q.bias;
+    p.act = q.act;
+    p.out_dt = q.out_dt;
+    p.out = q.out;
+    p.ldo = q.ldo;
+    // k over as many CTAs as there is room for, two k-blocks each at least
+    const int tiles = cdiv(q.n, 128);
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split * 2 <= 2 * sms && p.num_kb >= p.split * 4) p.split *= 2;
+    const CUtensorMap mw = tmap_2d_u8(q.w, q.n, q.k, q.ldw, 128);
+    const CUtensorMap mx = tmap_2d_u8(xq, q.rows, q.k, ldq, NT);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.split);
+    cfg.blockDim = dim3(kSkinnyThreads);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    M3R_CUDA(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
+}
+
 long long padded_k(int k) { return (static_cast<long long>(k) + 15) / 16 * 16; }
 size_t round256(size_t b) { return (b + 255) / 256 * 256; }
+
+// Up to 4 rows that fit the default shared memory of a block take the one-launch kernel.
+bool use_gemv(long long rows, int k) { return rows <= 4 && (rows == 3 ? 4 : rows) * padded_k(k) <= 40960; }
+
+template <int MR>
+void launch_gemv(cudaStream_t s, const Int8LinearParams& q, int sms) {
+    GemvParams p;
+    p.M = static_cast<int>(q.rows);
+    p.N = q.n;
+    p.K = q.k;
+    p.kpad = static_cast<int>(padded_k(q.k));
+    p.x_dt = q.x_dt;
+    p.out_dt = q.out_dt;
+    p.act = q.act;
+    p.x_vec = reinterpret_cast<uintptr_t>(q.x) % 16 == 0 && q.ldx * op_size(q.x_dt) % 16 == 0;
+    p.ldx = q.ldx;
+    p.ldw = q.ldw;
+    p.ldo = q.ldo;
+    p.x = q.x;
+    p.x_scale = q.x_scale;
+    p.w = q.w;
+    p.ws = q.w_scale;
+    p.bias = q.bias;
+    p.out = q.out;
+    const int blocks = cdiv(q.n, kGemvCols * (kGemvThreads / 32));
+    const int most = 2 * sms;
+    int8_gemv_kernel<MR><<<blocks < most ? blocks : most, kGemvThreads, MR * p.kpad, s>>>(p);
+    M3R_CUDA(cudaGetLastError());
+}
 
 }  // namespace
 
 // 8-bit rows of x, then their scales.
 size_t int8_linear_workspace(int x_dt, long long rows, int n, int k) {
     (void)n;
-    if (x_dt == OP_I8 || rows == 0) return 0;
+    if (x_dt == OP_I8 || rows == 0 || use_gemv(rows, k)) return 0;
     return round256(static_cast<size_t>(rows) * padded_k(k)) + round256(static_cast<size_t>(rows) * 4);
 }
 
 void int8_linear(cudaStream_t s, const Int8LinearParams& p) {
     if (p.rows == 0) return;
+    int dev = 0;
+    M3R_CUDA(cudaGetDevice(&dev));
+    const int sms = sm_count(dev);
+    if (use_gemv(p.rows, p.k)) {
+        if (p.rows == 1) return launch_gemv<1>(s, p, sms);
+        if (p.rows == 2) return launch_gemv<2>(s, p, sms);
+        return launch_gemv<4>(s, p, sms);
+    }
     const int8_t* xq = static_cast<const int8_t*>(p.x);
     long long ldq = p.ldx;
     const float* xs = p.x_scale;
@@ -588,16 +676,18 @@ void int8_linear(cudaStream_t s, const Int8LinearParams& p) {
         ldq = padded_k(p.k);
         xs = sc;
     }
-    int dev = 0;
-    M3R_CUDA(cudaGetDevice(&dev));
-    const int sms = sm_count(dev);
+    // few rows: the weights' bytes are the work
+    if (p.rows <= 16) return launch_skinny<16>(s, p, xq, ldq, xs, sms);
+    if (p.rows <= 32) return launch_skinny<32>(s, p, xq, ldq, xs, sms);
+    if (p.rows <= 64) return launch_skinny<64>(s, p, xq, ldq, xs, sms);
+    if (p.rows <= 128) return launch_skinny<128>(s, p, xq, ldq, xs, sms);
     // the largest tile that gives every SM one
     if (static_cast<long long>(cdiv(p.rows, 256)) * cdiv(p.n, 256) * 2 >= sms)
-        launch<256, 2>(s, p, xq, ldq, xs);
+        launch<256, 2>(s, p, xq, ldq, xs, sms);
     else if (static_cast<long long>(cdiv(p.rows, 128)) * cdiv(p.n, 128) >= sms)
-        launch<128, 1>(s, p, xq, ldq, xs);
+        launch<128, 1>(s, p, xq, ldq, xs, sms);
     else
-        launch<64, 1>(s, p, xq, ldq, xs);
+        launch<64, 1>(s, p, xq, ldq, xs, sms);
 }
 
 int int8_linear_status(cudaStream_t s) {

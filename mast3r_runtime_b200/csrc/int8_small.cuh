@@ -1,0 +1,395 @@
+// The 8-bit product for few rows of x, where the weights' bytes are the work.
+//
+// int8_gemv_kernel (up to 4 rows): one launch for everything.  Every block quantises the rows
+// itself, into shared memory, while its first weights travel; a warp takes 4 output channels at a
+// time, its lanes 16 bytes of k each, and adds up four products an instruction.
+//
+// int8_skinny_kernel (up to 128 rows): the roles of the operands are exchanged -- 128 output
+// channels are the rows of the tensor-core tile, the tokens its NT columns -- so that a stage of
+// the pipeline is mostly weights.  A cluster of up to 8 CTAs splits k; each leaves its sums in
+// shared memory, and every CTA adds and finishes some of the tokens from all of them (integer
+// sums: the order does not matter).
+#pragma once
+
+#include "common.cuh"
+#include "gemm.cuh"
+#include "ops.h"
+#include "quantize.cuh"
+
+namespace m3r {
+
+namespace {
+
+// y = act(acc * xs * ws + bias), one value
+__device__ __forceinline__ float finish1(int acc, float xs, float ws, float bias, int act, bool f32) {
+    const float v = fmaf(static_cast<float>(acc) * xs, ws, bias);
+    if (act == ACT_GELU) {
+        const float u = v * fmaf(v * v, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
+        if (f32) return v * __frcp_rn(1.0f + ex2_approx(-2.885390081777927f * u));
+        float t;
+        asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
+        return fmaf(0.5f * v, t, 0.5f * v);
+    }
+    if (act == ACT_RELU) return v < 0.0f ? 0.0f : v;  // keeps NaN
+    return v;
+}
+
+__device__ __forceinline__ void store1(void* out, int dt, long long at, float v) {
+    if (dt == OP_F32)
+        static_cast<float*>(out)[at] = v;
+    else if (dt == OP_F16)
+        static_cast<__half*>(out)[at] = __float2half_rn(v);
+    else
+        static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+}
+
+struct GemvParams {
+    int M, N, K, kpad;  // kpad: K rounded up to 16
+    int x_dt, out_dt, act, x_vec;
+    long long ldx, ldw, ldo;
+    const void* x;
+    const float* x_scale;
+    const int8_t* w;
+    const float* ws;
+    const float* bias;
+    void* out;
+};
+
+constexpr int kGemvThreads = 256;
+constexpr int kGemvCols = 4;
+
+// Eight values of a row from element e on (zero behind its end).
+template <class T>
+__device__ __forceinline__ void gemv_load8(const T* row, int e, int K, bool vec, float (&v)[8]) {
+    if (vec && e + 8 <= K) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(row + e));
+            const float4 b = __ldg(reinterpret_cast<const float4*>(row + e) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + e));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = Elem<T>::unpack(w[j]);
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = e + j < K ? to_f(row[e + j]) : 0.0f;
+    }
+}
+
+// Rows of x quantised into shared memory (zero behind their end), their scales into `scale`.
+template <class T, int MR>
+__device__ __forceinline__ void gemv_quantise(const GemvParams& p, uint8_t* sx, float* scale, uint32_t (*part)[MR]) {
+    const int tid = threadIdx.x;
+    const T* x = static_cast<const T*>(p.x);
+    uint32_t top[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+        float big = 0.0f;
+        if (m < p.M)
+            for (int e = tid * 8; e < p.K; e += kGemvThreads * 8) {
+                float v[8];
+                gemv_load8(x + m * p.ldx, e, p.K, p.x_vec, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) big = max_abs(big, v[j]);
+            }
+        top[m] = __reduce_max_sync(0xffffffffu, __float_as_uint(big) & 0x7FFFFFFFu);
+        if ((tid & 31) == 0) part[tid >> 5][m] = top[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+        uint32_t t = 0;
+#pragma unroll
+        for (int w = 0; w < kGemvThreads / 32; ++w) t = max(t, part[w][m]);
+        const bool live = live_magnitude(t);
+        const Quantizer z(__uint_as_float(t));
+        if (tid == m) scale[m] = z.a / 127.0f;
+        for (int e = tid * 8; e < p.kpad; e += kGemvThreads * 8) {
+            uint2 q = make_uint2(0, 0);
+            if (m < p.M && live) {
+                float v[8];
+                gemv_load8(x + m * p.ldx, e, p.K, p.x_vec, v);
+                q = quantize8<sizeof(T) == 2>(v, z);
+            }
+            *reinterpret_cast<uint2*>(sx + m * p.kpad + e) = q;
+        }
+    }
+}
+
+template <int MR>
+__global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_constant__ GemvParams p) {
+    extern __shared__ __align__(16) uint8_t sx[];  // [MR][kpad]
+    __shared__ float scale[MR];
+    __shared__ uint32_t part[kGemvThreads / 32][MR];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warps = gridDim.x * (kGemvThreads / 32);
+    const int chunks = p.K / 16, tail = p.K % 16;  // whole 16 bytes of k, and what is left
+    int n0 = (blockIdx.x * (kGemvThreads / 32) + (tid >> 5)) * kGemvCols;
+
+    // two steps of 16 bytes a lane for each channel; channels past the end read the last one
+    uint4 w[kGemvCols][2];
+    auto channel = [&](int i) { return p.w + static_cast<long long>(min(n0 + i, p.N - 1)) * p.ldw; };
+    auto load = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < kGemvCols; ++i) {
+            const uint4* row = reinterpret_cast<const uint4*>(channel(i));
+#pragma unroll
+            for (int s = 0; s < 2; ++s) w[i][s] = c + 32 * s < chunks ? __ldg(row + c + 32 * s) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (n0 < p.N) load(lane);
+    if (p.x_dt == OP_I8) {
+        for (int m = 0; m < MR; ++m) {
+            const int8_t* row = static_cast<const int8_t*>(p.x) + m * p.ldx;
+            for (int c = tid; c < chunks; c += kGemvThreads)
+                reinterpret_cast<uint4*>(sx + m * p.kpad)[c] =
+                    m < p.M ? __ldg(reinterpret_cast<const uint4*>(row) + c) : make_uint4(0, 0, 0, 0);
+            if (tid < tail) sx[m * p.kpad + chunks * 16 + tid] = m < p.M ? static_cast<uint8_t>(row[chunks * 16 + tid]) : 0;
+        }
+        if (tid < MR) scale[tid] = tid < p.M ? __ldg(p.x_scale + tid) : 0.0f;
+    } else if (p.x_dt == OP_F32) {
+        gemv_quantise<float, MR>(p, sx, scale, part);
+    } else if (p.x_dt == OP_F16) {
+        gemv_quantise<__half, MR>(p, sx, scale, part);
+    } else {
+        gemv_quantise<__nv_bfloat16, MR>(p, sx, scale, part);
+    }
+    __syncthreads();
+
+    while (n0 < p.N) {
+        int acc[kGemvCols][MR] = {};
+        const int8_t* last[kGemvCols];
+        if (tail) {
+#pragma unroll
+            for (int i = 0; i < kGemvCols; ++i) last[i] = channel(i) + chunks * 16;
+        }
+        const int first = n0;
+        for (int c = lane; c - lane < chunks; c += 64) {
+            uint4 a[kGemvCols][2];
+#pragma unroll
+            for (int i = 0; i < kGemvCols; ++i) a[i][0] = w[i][0], a[i][1] = w[i][1];
+            // the next weights travel while these are multiplied
+            if (c - lane + 64 < chunks) {
+                load(c + 64);
+            } else {
+                n0 += warps * kGemvCols;
+                if (n0 < p.N) load(lane);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (c + 32 * s < chunks) {
+#pragma unroll
+                    for (int m = 0; m < MR; ++m) {
+                        const int4 v = *reinterpret_cast<const int4*>(sx + m * p.kpad + (c + 32 * s) * 16);
+#pragma unroll
+                        for (int i = 0; i < kGemvCols; ++i) {
+                            acc[i][m] = __dp4a(static_cast<int>(a[i][s].x), v.x, acc[i][m]);
+                            acc[i][m] = __dp4a(static_cast<int>(a[i][s].y), v.y, acc[i][m]);
+                            acc[i][m] = __dp4a(static_cast<int>(a[i][s].z), v.z, acc[i][m]);
+                            acc[i][m] = __dp4a(static_cast<int>(a[i][s].w), v.w, acc[i][m]);
+                        }
+                    }
+                }
+            }
+        }
+        if (chunks == 0) n0 += warps * kGemvCols;
+        if (lane < tail) {
+#pragma unroll
+            for (int i = 0; i < kGemvCols; ++i)
+#pragma unroll
+                for (int m = 0; m < MR; ++m)
+                    acc[i][m] += static_cast<int>(last[i][lane]) *
+                                 static_cast<int>(static_cast<int8_t>(sx[m * p.kpad + chunks * 16 + lane]));
+        }
+        int mine = 0;  // lane i * MR + m finishes channel i of row m
+#pragma unroll
+        for (int i = 0; i < kGemvCols; ++i)
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                const int sum = __reduce_add_sync(0xffffffffu, acc[i][m]);
+                if (lane == i * MR + m) mine = sum;
+            }
+        const int n = first + lane / MR, m = lane % MR;
+        if (lane < kGemvCols * MR && n < p.N && m < p.M) {
+            const float b = p.bias ? __ldg(p.bias + n) : 0.0f;
+            store1(p.out, p.out_dt, m * p.ldo + n,
+                   finish1(mine, scale[m], __ldg(p.ws + n), b, p.act, p.out_dt == OP_F32));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------- skinny
+struct SkinnyParams {
+    int M, N, num_kb, split;  // k-blocks of 128 bytes, shared by `split` CTAs of a cluster
+    const float* xs;
+    const float* ws;
+    const float* bias;
+    int act, out_dt;
+    void* out;
+    long long ldo;
+};
+
+constexpr int kSkinnyThreads = 128;
+
+template <int NT>
+struct SkinnyCfg {
+    static constexpr int W_BYTES = 128 * 128;
+    static constexpr int X_BYTES = NT * 128;
+    static constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
+    // two CTAs an SM: about 100 KB each, and room for the 128 x NT sums in the same place
+    static constexpr int STAGES = 98304 / STAGE_BYTES;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+    static constexpr int TMEM_COLS = NT < 32 ? 32 : NT;
+    static_assert(NT * 128 * 4 <= STAGES * STAGE_BYTES, "the sums fit the stages' memory");
+    static_assert(X_BYTES % 1024 == 0, "operand tiles must be whole swizzle atoms");
+};
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t caddr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(caddr) : "memory");
+    return v;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kSkinnyThreads)
+    int8_skinny_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX,
+                       const __grid_constant__ SkinnyParams p) {
+    using C = SkinnyCfg<NT>;
+    constexpr int STAGES = C::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sW = smem;
+    uint8_t* sX = smem + STAGES * C::W_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* done = full + 2 * STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 2 * STAGES + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* err = &g_status.code;
+
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int split = p.split;
+    const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int n0 = (blockIdx.x / split) * 128;
+    const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / split);
+    const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / split);
+
+    if (tid == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&mapW);
+        prefetch_tmap(&mapX);
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (tid == 0) {
+        // ------------------------------------------------ TMA producer
+        bool ok = true;
+        int it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % STAGES;
+            if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, kDevTimeoutProducer, err)) {
+                ok = false;
+                break;
+            }
+            mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
+            tma_load_2d(sW + s * C::W_BYTES, &mapW, &full[s], kb * 128, n0);
+            tma_load_2d(sX + s * C::X_BYTES, &mapX, &full[s], kb * 128, 0);
+        }
+        if (!ok) {  // drain: wait (bounded) for loads that may still be in flight
+            volatile int dummy = 0;
+            for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j)
+                mbar_wait(&full[j % STAGES], (j / STAGES) & 1, &dummy, kDevTimeoutProducer, err);
+        }
+    } else if (tid == 32) {
+        // ------------------------------------------------ MMA issuer
+        constexpr uint32_t idesc = idesc_i8kind(128, NT);
+        int it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % STAGES;
+            if (!mbar_wait(&full[s], (it / STAGES) & 1, abort_flag, kDevTimeoutMma, err)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                mma_i8_ss(tmem, umma_desc_sw128(smem_u32(sW + s * C::W_BYTES) + k * 32, 16, 1024),
+                          umma_desc_sw128(smem_u32(sX + s * C::X_BYTES) + k * 32, 16, 1024), idesc,
+                          it > 0 || k > 0 ? 1u : 0u);
+            mma_commit(&empty[s]);
+        }
+        mma_commit(done);
+    }
+    __syncwarp();
+    // ------------------------------------------------ sums to shared memory: part[token][channel]
+    const int n = n0 + tid;
+    const float ws = n < p.N ? __ldg(p.ws + n) : 0.0f;
+    const float bias = n < p.N && p.bias ? __ldg(p.bias + n) : 0.0f;
+    {
+        volatile int dummy = 0;
+        mbar_wait(done, 0, &dummy, kDevTimeoutEpilogue, err);
+    }
+    tc_fence_after();
+    __syncthreads();  // every load has landed and been multiplied: the stages' memory is free
+    int* part = reinterpret_cast<int*>(smem);
+#pragma unroll 1
+    for (int c = 0; c < NT; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(c + i) * 128 + tid] = static_cast<int>(r[i]);
+    }
+    tc_fence_before();
+    if (split > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    // ------------------------------------------------ tokens rank, rank + split, ... of all sums
+    uint32_t peer[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) peer[r] = cluster_addr(smem_u32(part + tid), static_cast<uint32_t>(r < split ? r : 0));
+    for (int t0 = rank; t0 < p.M; t0 += 4 * split) {
+        int v[4][8];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                v[u][r] = r < split && t0 + u * split < p.M ? ld_cluster_s32(peer[r] + (t0 + u * split) * 512) : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int t = t0 + u * split;
+            int sum = 0;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) sum += v[u][r];
+            if (t < p.M && n < p.N)
+                store1(p.out, p.out_dt, t * p.ldo + n,
+                       finish1(sum, __ldg(p.xs + t), ws, bias, p.act, p.out_dt == OP_F32));
+        }
+    }
+    if (split > 1)
+        cluster_sync();  // no CTA leaves while another reads its sums
+    else
+        __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM_COLS);
+    }
+}
+
+}  // namespace
+
+}  // namespace m3r
