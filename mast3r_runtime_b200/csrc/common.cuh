@@ -446,6 +446,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// ---------------------------------------------------------------- dependent launches
+// A kernel launched as a programmatic dependent of the one before it on the stream starts once
+// every block of that one has called grid_dependency_start (or left), and sees its results after
+// grid_dependency_wait.  Both do nothing in ordinary launches.
+__device__ __forceinline__ void grid_dependency_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- numerics
 
 __device__ __forceinline__ float ex2_approx(float x) {

@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    grid_dependency_wait();  // rows quantised by the kernel before
     const uint32_t full_c = CG == 2 ? cluster_addr(smem_u32(full), 0) : smem_u32(full);
     const uint32_t tempty_c = CG == 2 ? cluster_addr(smem_u32(tempty), 0) : smem_u32(tempty);
     const uint32_t peer_abort_c =
@@ -510,6 +511,18 @@ int sm_count(int dev) {
     return n[dev];
 }
 
+// Cluster size, and after the rows' quantisation (a kernel of this call) a dependent launch: the
+// product sets up its barriers and TMEM, and fetches its first weights, while that one runs.
+int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster, const Int8LinearParams& q) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    return q.x_dt == OP_I8 ? 1 : 2;
+}
+
 // Raises a kernel's shared memory limit once on each device.
 template <class Kernel>
 void allow_smem(Kernel kern, int bytes, unsigned& done) {
@@ -555,13 +568,9 @@ void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long lo
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::SMEM_BYTES;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = launch_attributes(attr, CG, q);
     M3R_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, p));
 }
 
@@ -582,6 +591,7 @@ void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, 
     p.out_dt = q.out_dt;
     p.out = q.out;
     p.ldo = q.ldo;
+    p.out_vec = q.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(q.out) % (4 * op_size(q.out_dt)) == 0;
     // k over as many CTAs as there is room for, two k-blocks each at least
     const int tiles = cdiv(q.n, 128);
     p.split = 1;
@@ -593,13 +603,9 @@ void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, 
     cfg.blockDim = dim3(kSkinnyThreads);
     cfg.dynamicSmemBytes = C::SMEM_BYTES;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = launch_attributes(attr, p.split, q);
     M3R_CUDA(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
 }
 

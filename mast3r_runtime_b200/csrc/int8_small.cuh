@@ -230,7 +230,7 @@ struct SkinnyParams {
     const float* xs;
     const float* ws;
     const float* bias;
-    int act, out_dt;
+    int act, out_dt, out_vec;  // out_vec: 4 values of a row are an aligned access
     void* out;
     long long ldo;
 };
@@ -250,9 +250,12 @@ struct SkinnyCfg {
     static_assert(X_BYTES % 1024 == 0, "operand tiles must be whole swizzle atoms");
 };
 
-__device__ __forceinline__ int ld_cluster_s32(uint32_t caddr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(caddr) : "memory");
+__device__ __forceinline__ int4 ld_cluster_int4(uint32_t caddr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(caddr)
+                 : "memory");
     return v;
 }
 
@@ -299,9 +302,17 @@ __global__ void __launch_bounds__(kSkinnyThreads)
 
     if (tid == 0) {
         // ------------------------------------------------ TMA producer
+        // the first weights travel while the kernel before (the rows' quantisation) still runs
+        const int early = min(STAGES, kb1 - kb0);
+        for (int s = 0; s < early; ++s) {
+            mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
+            tma_load_2d(sW + s * C::W_BYTES, &mapW, &full[s], (kb0 + s) * 128, n0);
+        }
+        grid_dependency_wait();
+        for (int s = 0; s < early; ++s) tma_load_2d(sX + s * C::X_BYTES, &mapX, &full[s], (kb0 + s) * 128, 0);
         bool ok = true;
-        int it = 0;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        int it = early;
+        for (int kb = kb0 + early; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES;
             if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, kDevTimeoutProducer, err)) {
                 ok = false;
@@ -335,13 +346,19 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     }
     __syncwarp();
     // ------------------------------------------------ sums to shared memory: part[token][channel]
-    const int n = n0 + tid;
-    const float ws = n < p.N ? __ldg(p.ws + n) : 0.0f;
-    const float bias = n < p.N && p.bias ? __ldg(p.bias + n) : 0.0f;
+    const int lane = tid & 31;
+    float ws[4], bias[4];  // of the 4 channels that this thread finishes
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int n = n0 + 4 * lane + c;
+        ws[c] = n < p.N ? __ldg(p.ws + n) : 0.0f;
+        bias[c] = n < p.N && p.bias ? __ldg(p.bias + n) : 0.0f;
+    }
     {
         volatile int dummy = 0;
         mbar_wait(done, 0, &dummy, kDevTimeoutEpilogue, err);
     }
+    grid_dependency_wait();  // the rows' scales
     tc_fence_after();
     __syncthreads();  // every load has landed and been multiplied: the stages' memory is free
     int* part = reinterpret_cast<int*>(smem);
@@ -361,23 +378,44 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     // ------------------------------------------------ tokens rank, rank + split, ... of all sums
     uint32_t peer[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) peer[r] = cluster_addr(smem_u32(part + tid), static_cast<uint32_t>(r < split ? r : 0));
-    for (int t0 = rank; t0 < p.M; t0 += 4 * split) {
-        int v[4][8];
+    for (int r = 0; r < 8; ++r)
+        peer[r] = cluster_addr(smem_u32(part + 4 * lane), static_cast<uint32_t>(r < split ? r : 0));
+    constexpr int U = 2;  // tokens of a warp at once
+    for (int t0 = rank + split * warp; t0 < p.M; t0 += 4 * U * split) {
+        int4 v[U][8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                v[u][r] = r < split && t0 + u * split < p.M ? ld_cluster_s32(peer[r] + (t0 + u * split) * 512) : 0;
+            for (int r = 0; r < 8; ++r) {
+                const int t = t0 + u * 4 * split;
+                v[u][r] = r < split && t < p.M ? ld_cluster_int4(peer[r] + t * 512) : make_int4(0, 0, 0, 0);
+            }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int t = t0 + u * split;
-            int sum = 0;
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + u * 4 * split;
+            if (t >= p.M) continue;
+            int sum[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 8; ++r) sum += v[u][r];
-            if (t < p.M && n < p.N)
-                store1(p.out, p.out_dt, t * p.ldo + n,
-                       finish1(sum, __ldg(p.xs + t), ws, bias, p.act, p.out_dt == OP_F32));
+            for (int r = 0; r < 8; ++r) sum[0] += v[u][r].x, sum[1] += v[u][r].y, sum[2] += v[u][r].z, sum[3] += v[u][r].w;
+            const float xs = __ldg(p.xs + t);
+            float y[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = finish1(sum[c], xs, ws[c], bias[c], p.act, p.out_dt == OP_F32);
+            const long long at = t * p.ldo + n0 + 4 * lane;
+            if (p.out_vec && n0 + 4 * lane + 4 <= p.N) {
+                if (p.out_dt == OP_F32)
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
+                else if (p.out_dt == OP_F16)
+                    *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
+                        make_uint2(Elem<__half>::pack(y[0], y[1]), Elem<__half>::pack(y[2], y[3]));
+                else
+                    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+                        make_uint2(Elem<__nv_bfloat16>::pack(y[0], y[1]), Elem<__nv_bfloat16>::pack(y[2], y[3]));
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (n0 + 4 * lane + c < p.N) store1(p.out, p.out_dt, at + c, y[c]);
+            }
         }
     }
     if (split > 1)

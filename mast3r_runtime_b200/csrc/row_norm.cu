@@ -231,6 +231,7 @@ template <bool VEC, int NCH, bool WARP, int MODE, int GT>
 __global__ void __launch_bounds__(WARP ? 128 : VEC ? 1024 : GT, WARP && NCH == 4 && MODE == ROW_FULL ? 5 : 0) row_norm_kernel(const __grid_constant__ RowNormParams p) {
     constexpr int N = 8 * NCH;
     __shared__ float red_buf[64];
+    if constexpr (MODE != ROW_FULL) grid_dependency_start();  // the product that follows may set itself up
     RowReduce<WARP> red{red_buf, 0};
     const RowSlice<VEC, NCH, GT> s(WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
                                WARP ? 32 : VEC ? static_cast<int>(blockDim.x) : GT, p.cols);
