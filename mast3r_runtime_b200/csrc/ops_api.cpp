@@ -5,7 +5,6 @@
 #include <string>
 
 #include "../../include/m3r_cuda.h"
-#include "engine.h"
 #include "ops.h"
 #include "tmap.h"
 
@@ -34,6 +33,20 @@ int guarded(F&& fn) {
         return M3R_ERR_CUDA;
     }
 }
+
+// The call's device for the scope; leaves the runtime alone when it is current already.
+struct OpDevice {
+    int prev = 0;
+    bool set;
+    explicit OpDevice(int dev) {
+        M3R_CUDA(cudaGetDevice(&prev));
+        set = prev != dev;
+        if (set) M3R_CUDA(cudaSetDevice(dev));
+    }
+    ~OpDevice() {
+        if (set) cudaSetDevice(prev);
+    }
+};
 
 bool is_float(int dt) { return dt == M3R_DTYPE_BF16 || dt == M3R_DTYPE_F16 || dt == M3R_DTYPE_F32; }
 
@@ -81,7 +94,7 @@ int m3r_quantize_rows(const m3r_quantize_args* args) {
     return guarded([&] {
         M3R_REQUIRE(args != nullptr, "quantize_rows: null arguments");
         const m3r::RowNormParams p = quantize_params(*args);
-        m3r::DeviceGuard g(args->device);
+        OpDevice g(args->device);
         m3r::row_norm(static_cast<cudaStream_t>(args->stream), p);
     });
 }
@@ -148,7 +161,7 @@ int m3r_int8_linear(const m3r_int8_linear_args* args) {
         p.bias = a.bias;
         p.out = a.out;
         p.workspace = a.workspace;
-        m3r::DeviceGuard g(a.device);
+        OpDevice g(a.device);
         m3r::int8_linear(static_cast<cudaStream_t>(a.stream), p);
     });
 }
@@ -213,7 +226,7 @@ int m3r_residual_norm(const m3r_residual_norm_args* args) {
         p.r = a.r;
         p.out = a.out;
         p.out_scale = a.out_scale;
-        m3r::DeviceGuard g(a.device);
+        OpDevice g(a.device);
         m3r::row_norm(static_cast<cudaStream_t>(a.stream), p);
     });
 }
@@ -274,14 +287,14 @@ int m3r_rope(const m3r_rope_args* args) {
         p.pos_axis = a.pos_axis;
         p.pos_b = a.pos_batch;
         p.pos_t = a.pos_token;
-        m3r::DeviceGuard g(a.device);
+        OpDevice g(a.device);
         m3r::rope(static_cast<cudaStream_t>(a.stream), p);
     });
 }
 
 int m3r_operator_status(int device, void* stream) {
     return guarded([&] {
-        m3r::DeviceGuard g(device);
+        OpDevice g(device);
         const int code = m3r::int8_linear_status(static_cast<cudaStream_t>(stream));
         if (code) throw m3r::Error(m3r::kErrTimeout, "device wait timed out (code " + std::to_string(code) + ")");
     });

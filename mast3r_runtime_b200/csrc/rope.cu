@@ -14,6 +14,8 @@
 // and 194 us instead of 130).  Angles are reduced in 64 bits -- position * (inv_freq / 2 pi)
 // minus its nearest integer -- so that a far position keeps its fraction of a turn: in 32
 // bits position 1e6 would leave it with 2^-5 of a radian.
+#include <algorithm>
+
 #include "common.cuh"
 #include "ops.h"
 #include "tmap.h"
@@ -24,7 +26,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxAngles = 2048;  // sines and cosines of a block: 16 KB
-constexpr int kMaxTokens = 32;    // tokens of a block
+constexpr int kMaxTokens = 64;    // tokens of a block
+constexpr int kBlocksPerSm = 6;
 
 struct RopeGrid {
     int tokens_per_block, heads_per_block, head_blocks, head_chunks;
@@ -58,7 +61,7 @@ __device__ __forceinline__ T put_f(float x) {
 // accesses each), the adjacent one 2 n_freq / VE of VE / 2 pairs; then the chunks of the tail.
 // VE = 1 of the adjacent layout takes a pair a chunk.
 template <class T, int VE, bool ADJ>
-__global__ void __launch_bounds__(kThreads, 6) rope_kernel(const __grid_constant__ RopeParams p,
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __grid_constant__ RopeParams p,
                                                         const __grid_constant__ RopeGrid g) {
     using V = Pack<T, VE>;
     constexpr int PAIRS = ADJ ? (VE > 1 ? VE / 2 : 1) : VE;  // pairs a chunk
@@ -164,19 +167,28 @@ void launch(cudaStream_t s, const RopeParams& p) {
     RopeGrid g;
     g.head_chunks = p.n_freq / PAIRS + (p.dim - 2 * p.n_freq) / VE;
     g.cols = g.head_chunks < kThreads ? g.head_chunks : kThreads;
-    // tokens a block: 8 accesses for every thread (2 to 16 measured, on 98,304 tokens of 32 heads of 64:
-    // 148, 135, 130, 134 us); while there are few tokens, fewer, and then the heads split over blocks
-    // (each computes its tokens' sines)
+    // Tokens a block: a block costs its accesses a thread and some for its start (98,304 tokens of 32
+    // heads of 64, with 2, 4, 8 and 16 accesses: 148, 135, 130, 134 us); while there are few blocks, the
+    // last round of them over the SMs counts whole.  With few tokens the heads are split over blocks, and
+    // each computes its tokens' sines.
     const int rows = kThreads / g.cols;
-    g.tokens_per_block = rows * 8 / heads > 1 ? rows * 8 / heads : 1;
-    if (g.tokens_per_block > kMaxTokens) g.tokens_per_block = kMaxTokens;
-    if (g.tokens_per_block > kMaxAngles / p.n_freq) g.tokens_per_block = kMaxAngles / p.n_freq;
-    while (g.tokens_per_block > 1 && all / g.tokens_per_block < 4 * 148) g.tokens_per_block /= 2;
+    const long long slots = 148LL * kBlocksPerSm;
+    const int most = static_cast<int>(std::min<long long>({kMaxTokens, kMaxAngles / p.n_freq, all}));
+    g.tokens_per_block = 1;
+    double best = 0;
+    for (int t = 1; t <= most; ++t) {
+        const long long blocks = (all + t - 1) / t;
+        const double rounds = blocks >= 4 * slots ? static_cast<double>(blocks) / slots + 0.5 : (blocks + slots - 1) / slots;
+        const double cost = rounds * ((t * heads + rows - 1) / rows + 0.4);
+        if (t == 1 || cost < best) {
+            best = cost;
+            g.tokens_per_block = t;
+        }
+    }
     const long long token_blocks = (all + g.tokens_per_block - 1) / g.tokens_per_block;
     g.heads_per_block = heads;
-    const long long want = 4 * 148;
-    if (token_blocks < want) {
-        const long long split = want / token_blocks < heads ? want / token_blocks : heads;
+    if (g.tokens_per_block == 1 && token_blocks < slots) {
+        const long long split = slots / token_blocks < heads ? slots / token_blocks : heads;
         g.heads_per_block = static_cast<int>((heads + split - 1) / split);
         // at least one access for every thread
         if (g.heads_per_block < rows) g.heads_per_block = rows < heads ? rows : heads;

@@ -9,7 +9,7 @@
 // a = max |h|, q = the integer nearest to 127 h / a (ties to even), scale = a / 127.
 //
 // The work is bound by HBM: x, y in, r, h out, each once.  A row of at most 1,024 values
-// belongs to one warp (statistics by shuffles, no block barrier), a longer one to one
+// belongs to one warp or a part of one (statistics by shuffles, no block barrier), a longer one to one
 // block; x and y are loaded before the first reduction so that a warp keeps its whole
 // row's bytes in flight.  All statistics are 32-bit, the variance in two passes over the
 // registers.
@@ -133,16 +133,21 @@ struct RowSlice {
     }
 };
 
-// Sum / maximum over the threads of a row: a warp's shuffles, then one word of each warp.
-// `buf` alternates between two halves so that one barrier a reduction is enough.
-template <bool WARP>
+// Sum / maximum over the LANES threads of a row in a warp (shuffles), or, with LANES = 0, over a
+// block: a warp's shuffles, then one word of each warp.  `buf` alternates between two halves so
+// that one barrier a reduction is enough.
+template <int LANES>
 struct RowReduce {
     float* buf;  // [2][32]
     int flip;
+    unsigned mask;  // the row's lanes: rows of a warp may end in different rounds
+    __device__ __forceinline__ explicit RowReduce(float* b) : buf(b), flip(0), mask(0xffffffffu) {
+        if constexpr (LANES > 0 && LANES < 32) mask = ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);
+    }
     __device__ __forceinline__ float sum(float v) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if constexpr (!WARP) {
+        for (int o = LANES ? LANES / 2 : 16; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+        if constexpr (LANES == 0) {
             float* at = buf + 32 * flip;
             flip ^= 1;
             if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
@@ -155,8 +160,13 @@ struct RowReduce {
         return v;
     }
     __device__ __forceinline__ uint32_t max(uint32_t v) {
+        if constexpr (LANES > 0 && LANES < 32) {
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) v = ::max(v, __shfl_xor_sync(mask, v, o));
+            return v;
+        }
         v = __reduce_max_sync(0xffffffffu, v);
-        if constexpr (!WARP) {
+        if constexpr (LANES == 0) {
             uint32_t* at = reinterpret_cast<uint32_t*>(buf + 32 * flip);
             flip ^= 1;
             if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
@@ -168,8 +178,8 @@ struct RowReduce {
     }
 };
 
-template <bool VEC, int NCH, bool WARP, int GT>
-__device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowReduce<WARP>& red, float (&v)[8 * NCH],
+template <bool VEC, int NCH, int LANES, int GT>
+__device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowReduce<LANES>& red, float (&v)[8 * NCH],
                                           int kind, float eps, const float* w, const float* b) {
     constexpr int N = 8 * NCH;
     const float inv_d = 1.0f / static_cast<float>(s.D);
@@ -198,8 +208,8 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowRe
     }
 }
 
-template <bool EXACT16, bool VEC, int NCH, bool WARP, int GT>
-__device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH, GT>& s, RowReduce<WARP>& red, const float (&v)[8 * NCH],
+template <bool EXACT16, bool VEC, int NCH, int LANES, int GT>
+__device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH, GT>& s, RowReduce<LANES>& red, const float (&v)[8 * NCH],
                                            int8_t* q, float* scale) {
     constexpr int N = 8 * NCH;
     float m = 0.0f;
@@ -227,16 +237,19 @@ __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH, GT>& s, RowR
 // rows in flight: an SM needs about 40 KB of loads under way).
 enum RowMode : int { ROW_FULL = 0, ROW_QUANTIZE_F32 = 1, ROW_QUANTIZE_16 = 2 };
 
-template <bool VEC, int NCH, bool WARP, int MODE, int GT>
-__global__ void __launch_bounds__(WARP ? 128 : VEC ? 1024 : GT, WARP && NCH == 4 && MODE == ROW_FULL ? 5 : 0) row_norm_kernel(const __grid_constant__ RowNormParams p) {
+// LANES threads of a warp to a row (a few rows to a warp when it is short), or 0: a block.
+template <bool VEC, int NCH, int LANES, int MODE, int GT>
+__global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH == 4 && MODE == ROW_FULL ? 5 : 0)
+    row_norm_kernel(const __grid_constant__ RowNormParams p) {
     constexpr int N = 8 * NCH;
-    __shared__ float red_buf[64];
     if constexpr (MODE != ROW_FULL) grid_dependency_start();  // the product that follows may set itself up
-    RowReduce<WARP> red{red_buf, 0};
-    const RowSlice<VEC, NCH, GT> s(WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x),
-                               WARP ? 32 : VEC ? static_cast<int>(blockDim.x) : GT, p.cols);
-    const long long per = WARP ? blockDim.x >> 5 : 1;
-    for (long long row = blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); row < p.rows; row += gridDim.x * per) {
+    __shared__ float red_buf[64];
+    RowReduce<LANES> red(red_buf);
+    const int tid = LANES ? static_cast<int>(threadIdx.x % (LANES ? LANES : 1)) : static_cast<int>(threadIdx.x);
+    const RowSlice<VEC, NCH, GT> s(tid, LANES ? LANES : VEC ? static_cast<int>(blockDim.x) : GT, p.cols);
+    const int per = LANES ? static_cast<int>(blockDim.x) / (LANES ? LANES : 1) : 1;
+    const long long first = static_cast<long long>(blockIdx.x) * per + (LANES ? threadIdx.x / (LANES ? LANES : 1) : 0);
+    for (long long row = first; row < p.rows; row += static_cast<long long>(gridDim.x) * per) {
         float v[N];
         s.load_dt(p.x_dt, p.x, row * p.ldx, v);
         if constexpr (MODE != ROW_FULL) {
@@ -275,15 +288,15 @@ __global__ void __launch_bounds__(WARP ? 128 : VEC ? 1024 : GT, WARP && NCH == 4
     }
 }
 
-template <bool VEC, int NCH, bool WARP, int GT = 0>
+template <bool VEC, int NCH, int LANES, int GT = LANES>
 void launch(cudaStream_t s, const RowNormParams& p, int threads) {
-    const long long per = WARP ? threads / 32 : 1;
+    const long long per = LANES ? threads / (LANES ? LANES : 1) : 1;
     long long grid = (p.rows + per - 1) / per;
     if (grid > 148 * 64) grid = 148 * 64;
     const bool full = p.y != nullptr || p.r != nullptr || p.norm != NORM_NONE || p.out_dt != OP_I8 || p.alpha != 1.0f;
-    auto kern = full                ? row_norm_kernel<VEC, NCH, WARP, ROW_FULL, GT>
-                : p.x_dt == OP_F32 ? row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_F32, GT>
-                                   : row_norm_kernel<VEC, NCH, WARP, ROW_QUANTIZE_16, GT>;
+    auto kern = full                ? row_norm_kernel<VEC, NCH, LANES, ROW_FULL, GT>
+                : p.x_dt == OP_F32 ? row_norm_kernel<VEC, NCH, LANES, ROW_QUANTIZE_F32, GT>
+                                   : row_norm_kernel<VEC, NCH, LANES, ROW_QUANTIZE_16, GT>;
     kern<<<static_cast<int>(grid), threads, 0, s>>>(p);
     M3R_CUDA(cudaGetLastError());
 }
@@ -292,31 +305,37 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * op_size(dt)) % bytes == 0);
 }
 
-// Rows to warps or blocks.  With many rows, a warp each up to 1,024 values (98,304 rows of 1,024,
-// 32-bit stream: 199 us, against 226 with a block each); with few, a block each, 8 values a
-// thread, so that a row's chain of loads and reductions is short (1,536 rows of 1,024 quantised:
-// 4.0 us against 6.8).
+// Rows to threads.  Short rows share a warp, 8 values a lane.  With many rows, a warp each up to
+// 1,024 values (98,304 rows of 1,024, 32-bit stream: 199 us, against 226 with a block each); with
+// few, a block each, 8 values a thread, so that a row's chain of loads and reductions is short
+// (1,536 rows of 1,024 quantised: 4.0 us against 6.8).
 void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
-    if (p.cols <= 256) return launch<true, 1, true>(s, p, 128);
+    if (p.cols <= 32) return launch<true, 1, 4>(s, p, 128);
+    if (p.cols <= 64) return launch<true, 1, 8>(s, p, 128);
+    if (p.cols <= 128) return launch<true, 1, 16>(s, p, 128);
+    if (p.cols <= 256) return launch<true, 1, 32>(s, p, 128);
     if (p.rows > 148 * 16) {
-        if (p.cols <= 512) return launch<true, 2, true>(s, p, 128);
-        if (p.cols <= 1024) return launch<true, 4, true>(s, p, 128);
+        if (p.cols <= 512) return launch<true, 2, 32>(s, p, 128);
+        if (p.cols <= 1024) return launch<true, 4, 32>(s, p, 128);
     }
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
-    if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, false>(s, p, threads(1));
-    launch<true, 2, false>(s, p, threads(2));
+    if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, 0>(s, p, threads(1));
+    launch<true, 2, 0>(s, p, threads(2));
 }
 
 // Element accesses (odd widths, rows off the 16-byte grid): 8 values a thread, neighbouring
 // threads at neighbouring elements.
 void dispatch_elements(cudaStream_t s, const RowNormParams& p) {
-    if (p.cols <= 256) return launch<false, 1, true, 32>(s, p, 128);
-    if (p.cols <= 512) return launch<false, 1, false, 64>(s, p, 64);
-    if (p.cols <= 1024) return launch<false, 1, false, 128>(s, p, 128);
-    if (p.cols <= 2048) return launch<false, 1, false, 256>(s, p, 256);
-    if (p.cols <= 4096) return launch<false, 1, false, 512>(s, p, 512);
-    if (p.cols <= 8192) return launch<false, 1, false, 1024>(s, p, 1024);
-    launch<false, 2, false, 1024>(s, p, 1024);
+    if (p.cols <= 32) return launch<false, 1, 4>(s, p, 128);
+    if (p.cols <= 64) return launch<false, 1, 8>(s, p, 128);
+    if (p.cols <= 128) return launch<false, 1, 16>(s, p, 128);
+    if (p.cols <= 256) return launch<false, 1, 32>(s, p, 128);
+    if (p.cols <= 512) return launch<false, 1, 0, 64>(s, p, 64);
+    if (p.cols <= 1024) return launch<false, 1, 0, 128>(s, p, 128);
+    if (p.cols <= 2048) return launch<false, 1, 0, 256>(s, p, 256);
+    if (p.cols <= 4096) return launch<false, 1, 0, 512>(s, p, 512);
+    if (p.cols <= 8192) return launch<false, 1, 0, 1024>(s, p, 1024);
+    launch<false, 2, 0, 1024>(s, p, 1024);
 }
 
 }  // namespace

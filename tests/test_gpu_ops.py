@@ -256,7 +256,7 @@ def check_residual(ops, x, y, w, b, norm, out, **kw):
     return r, h
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 33), (4, 256), (7, 384), (130, 1000), (65, 1001), (64, 1024),
+@pytest.mark.parametrize("rows,cols", [(1, 1), (9, 8), (1003, 32), (70, 31), (41, 64), (77, 100), (35, 128), (3, 33), (4, 256), (7, 384), (130, 1000), (65, 1001), (64, 1024),
                                        (5, 1032), (301, 4096), (2, 4096), (3, 8191), (2, 16384)])
 @pytest.mark.parametrize("norm,post", [("layer", None), ("rms", "rms"), ("layer", "layer")])
 def test_residual_norm(ops, rows, cols, norm, post):
@@ -296,7 +296,7 @@ def test_residual_norm_types_and_gates(ops, stream, branch):
     assert torch.equal(wide, keep)  # nothing beside the rows was written
 
 
-@pytest.mark.parametrize("cols", [64, 1000, 1001, 4096])
+@pytest.mark.parametrize("cols", [24, 64, 65, 120, 1000, 1001, 4096])
 def test_residual_norm_in_8_bits(ops, cols):
     x, y = rnd(33, cols, seed=1), rnd(33, cols, seed=2, dtype=torch.bfloat16)
     x[5] = 0
