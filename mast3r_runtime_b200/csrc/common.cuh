@@ -135,6 +135,15 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16; both addresses 16-byte aligned) into this CTA's shared
+// memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // ---------------------------------------------------------------- CTA pairs (cluster of 2)
 // In a CTA pair the even CTA (rank 0) issues the MMAs; the TMA loads of both
 // CTAs signal its "full" barriers (the .cta_group::2 form lets the barrier be in

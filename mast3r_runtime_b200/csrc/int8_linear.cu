@@ -10,10 +10,9 @@
 // 128 x BN (one CTA) or 256 x BN (a CTA pair, cta_group::2), k in blocks of 128 bytes (one
 // swizzle atom a row), accumulators double-buffered in TMEM so that the epilogue of a tile
 // overlaps the main loop of the next.
-#include <mutex>
-
 #include "common.cuh"
 #include "gemm.cuh"
+#include "launch.h"
 #include "ops.h"
 #include "tmap.h"
 
@@ -521,18 +520,6 @@ int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster, const Int8Lin
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     return q.x_dt == OP_I8 ? 1 : 2;
-}
-
-// Raises a kernel's shared memory limit once on each device.
-template <class Kernel>
-void allow_smem(Kernel kern, int bytes, unsigned& done) {
-    int dev = 0;
-    M3R_CUDA(cudaGetDevice(&dev));
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev < 32 && (done >> dev & 1)) return;
-    M3R_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (dev < 32) done |= 1u << dev;
 }
 
 template <int BN, int CG>

@@ -37,6 +37,9 @@ struct RowNormParams {
     float* out_scale;   // rows of an 8-bit result
 };
 void row_norm(cudaStream_t s, const RowNormParams& p);
+// Code of the first device wait of a row kernel that ran out on the current device (0: none), read
+// after the stream's work; clears it.
+int row_norm_status(cudaStream_t s);
 
 // Rotary positions on up to two tensors [batch, tokens, heads, dim].
 struct RopeTensor {
@@ -73,8 +76,7 @@ struct Int8LinearParams {
 };
 size_t int8_linear_workspace(int x_dt, long long rows, int n, int k);
 void int8_linear(cudaStream_t s, const Int8LinearParams& p);
-// Code of the first device wait of an operator that ran out on the current device (0: none),
-// read after the stream's work; clears it.
+// The same for the product's kernels.
 int int8_linear_status(cudaStream_t s);
 
 }  // namespace m3r

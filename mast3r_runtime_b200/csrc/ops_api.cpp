@@ -295,7 +295,9 @@ int m3r_rope(const m3r_rope_args* args) {
 int m3r_operator_status(int device, void* stream) {
     return guarded([&] {
         OpDevice g(device);
-        const int code = m3r::int8_linear_status(static_cast<cudaStream_t>(stream));
+        const int product = m3r::int8_linear_status(static_cast<cudaStream_t>(stream));
+        const int rows = m3r::row_norm_status(static_cast<cudaStream_t>(stream));
+        const int code = product ? product : rows;
         if (code) throw m3r::Error(m3r::kErrTimeout, "device wait timed out (code " + std::to_string(code) + ")");
     });
 }

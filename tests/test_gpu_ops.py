@@ -270,6 +270,25 @@ def test_residual_norm(ops, rows, cols, norm, post):
                    residual_scale=0.75, **kw)
 
 
+@pytest.mark.parametrize("rows,cols,stream,branch", [(2400, 1536, "fp32", "bf16"), (1300, 4096, "bf16", "fp16"),
+                                                     (300, 16384, "fp32", "fp32"), (640, 8192, "fp16", "fp16")])
+def test_residual_norm_many_long_rows(ops, rows, cols, stream, branch):
+    """More rows than blocks fit the device: each block works through several, some copied ahead."""
+    x, y = rnd(rows, cols, seed=1, dtype=DT[stream]), rnd(rows, cols, seed=2, dtype=DT[branch])
+    w, b = 1 + 0.1 * rnd(cols, seed=1), 0.1 * rnd(cols, seed=2)
+    r, h = check_residual(ops, x, y, w, b, "layer", DT[branch], gate=rnd(cols, seed=5), post_norm="rms")
+    x2 = x.clone()
+    r2, h2 = ops.residual_norm(x2, y, w, b, norm="layer", out_dtype=DT[branch], gate=rnd(cols, seed=5), post_norm="rms",
+                               inplace=True)
+    assert r2 is x2 and torch.equal(r2, r) and torch.equal(h2, h)
+    q, s = ops.quantize_rows(x)
+    wq, wsc = levels(x)
+    assert torch.equal(q, wq) and torch.equal(s, wsc)
+    _, h3 = ops.residual_norm(x, None, w, None, norm="rms", out_dtype=torch.float32)
+    _, q3, s3 = ops.residual_norm(x, None, w, None, norm="rms", out_dtype=torch.int8)
+    assert torch.equal(q3, levels(h3)[0]) and torch.equal(s3, levels(h3)[1])
+
+
 @pytest.mark.parametrize("stream", DT)
 @pytest.mark.parametrize("branch", DT)
 def test_residual_norm_types_and_gates(ops, stream, branch):
