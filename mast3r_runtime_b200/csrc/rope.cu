@@ -29,8 +29,11 @@ constexpr int kMaxAngles = 2048;  // sines and cosines of a block: 16 KB
 constexpr int kMaxTokens = 64;    // tokens of a block
 constexpr int kBlocksPerSm = 6;
 
+constexpr int kMaxHeads = 256;    // heads of a block
+
 struct RopeGrid {
-    int tokens_per_block, heads_per_block, head_blocks, head_chunks;
+    int tokens_per_block, heads_per_block, head_blocks;
+    int rot_chunks, tail_chunks;
     int cols;  // threads along a head's chunks; kThreads / cols heads at a time
 };
 
@@ -57,21 +60,25 @@ __device__ __forceinline__ T put_f(float x) {
         return Elem<T>::from(x);
 }
 
-// Head chunks of one (token, head): the half layout has n_freq / VE chunks of VE pairs (two
-// accesses each), the adjacent one 2 n_freq / VE of VE / 2 pairs; then the chunks of the tail.
-// VE = 1 of the adjacent layout takes a pair a chunk.
+// A thread turns one chunk of a head -- VE pairs in the half layout (two accesses), VE / 2 in the
+// adjacent one (one; a single pair for VE = 1) -- and copies every `rot_chunks`-th chunk of the tail, so
+// that all lanes do the same.
 template <class T, int VE, bool ADJ>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __grid_constant__ RopeParams p,
-                                                        const __grid_constant__ RopeGrid g) {
+                                                                     const __grid_constant__ RopeGrid g) {
     using V = Pack<T, VE>;
     constexpr int PAIRS = ADJ ? (VE > 1 ? VE / 2 : 1) : VE;  // pairs a chunk
+    constexpr bool TWO = !ADJ || VE == 1;                    // a pair is split over two accesses
     __shared__ float2 turn[kMaxAngles];                      // [token][frequency]: amplitude * (cos, sin)
     __shared__ double place[kMaxTokens][2];                  // the token's position on each axis
     __shared__ long long base[kMaxTokens][4];                // its offsets in the inputs and outputs of both tensors
+    __shared__ const T* from[kMaxHeads];                     // where the block's heads start
+    __shared__ T* to[kMaxHeads];
     const int all = static_cast<int>(p.batch * p.tokens);
     const int tok0 = static_cast<int>(blockIdx.x / g.head_blocks) * g.tokens_per_block;
     const int head0 = static_cast<int>(blockIdx.x % g.head_blocks) * g.heads_per_block;
     const int heads = min(g.heads_per_block, p.t[0].heads + p.t[1].heads - head0);
+    const int split = p.t[0].heads - head0;  // the block's heads from here on are the second tensor's
     const int ntok = min(g.tokens_per_block, all - tok0);
     const int tid = threadIdx.x;
     if (tid < 2 * ntok) {
@@ -85,29 +92,25 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
                                       : static_cast<double>(static_cast<const int*>(p.pos)[at]);
         }
     }
+    for (int h = tid; h < heads; h += kThreads) {
+        const RopeTensor& x = p.t[h >= split];
+        const long long at = h >= split ? h - split : h + head0;
+        from[h] = static_cast<const T*>(x.x) + at * x.xh;
+        to[h] = static_cast<T*>(x.out) + at * x.oh;
+    }
     __syncthreads();
-    // a thread's work: chunk c of (token, head) pair j, then of pair j + rows, ...
     const int rows = kThreads / g.cols;
-    const int rot_chunks = p.n_freq / PAIRS;
     const int first = tid / g.cols;
+    const int step_t = rows / heads, step_h = rows - step_t * heads;
     const int pairs = first < rows ? ntok * heads : 0;
     int c = tid % g.cols, j = first, tk = first / heads, h = first - tk * heads;
-    bool tail, two;  // behind the front part; a pair split over two accesses
-    int e0, e1;
-    T* dst;
+    const T* src;
     V lo, hi;
     auto load = [&]() {
-        const int second = h + head0 >= p.t[0].heads;
-        const RopeTensor& x = p.t[second];
-        const long long hh = h + head0 - (second ? p.t[0].heads : 0);
-        const T* src = static_cast<const T*>(x.x) + base[tk][second] + hh * x.xh;
-        dst = static_cast<T*>(x.out) + base[tk][2 + second] + hh * x.oh;
-        tail = c >= rot_chunks;
-        two = !tail && (!ADJ || VE == 1);
-        e0 = tail ? 2 * p.n_freq + (c - rot_chunks) * VE : ADJ && VE == 1 ? 2 * c : c * VE;
-        e1 = ADJ ? e0 + 1 : p.n_freq + c * VE;
-        lo = *reinterpret_cast<const V*>(src + e0);
-        if (two) hi = *reinterpret_cast<const V*>(src + e1);
+        src = from[h] + base[tk][h >= split];
+        const T* at = src + (ADJ && VE == 1 ? 2 * c : c * VE);
+        lo = *reinterpret_cast<const V*>(at);
+        if (TWO) hi = *reinterpret_cast<const V*>(at + (ADJ ? 1 : p.n_freq));
     };
     bool live = j < pairs;
     if (live) load();  // travels while the sines are computed
@@ -120,31 +123,37 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
     }
     __syncthreads();
     while (live) {
-        if (!tail) {
-            const float2* w = turn + tk * p.n_freq + c * PAIRS;
-            if constexpr (!ADJ || VE == 1) {
+        T* dst = to[h] + base[tk][2 + (h >= split)];
+        // behind the front part
+        for (int e = c; e < g.tail_chunks; e += g.rot_chunks) {
+            const int at = 2 * p.n_freq + e * VE;
+            *reinterpret_cast<V*>(dst + at) = *reinterpret_cast<const V*>(src + at);
+        }
+        const float2* w = turn + tk * p.n_freq + c * PAIRS;
+        if constexpr (TWO) {
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const float a = get_f(lo.v[i]), b = get_f(hi.v[i]);
-                    const float2 r = w[i];
-                    lo.v[i] = put_f<T>(a * r.x - b * r.y);
-                    hi.v[i] = put_f<T>(a * r.y + b * r.x);
-                }
-            } else {
+            for (int i = 0; i < VE; ++i) {
+                const float a = get_f(lo.v[i]), b = get_f(hi.v[i]);
+                const float2 r = w[i];
+                lo.v[i] = put_f<T>(a * r.x - b * r.y);
+                hi.v[i] = put_f<T>(a * r.y + b * r.x);
+            }
+        } else {
 #pragma unroll
-                for (int i = 0; i < VE / 2; ++i) {
-                    const float a = get_f(lo.v[2 * i]), b = get_f(lo.v[2 * i + 1]);
-                    const float2 r = w[i];
-                    lo.v[2 * i] = put_f<T>(a * r.x - b * r.y);
-                    lo.v[2 * i + 1] = put_f<T>(a * r.y + b * r.x);
-                }
+            for (int i = 0; i < VE / 2; ++i) {
+                const float a = get_f(lo.v[2 * i]), b = get_f(lo.v[2 * i + 1]);
+                const float2 r = w[i];
+                lo.v[2 * i] = put_f<T>(a * r.x - b * r.y);
+                lo.v[2 * i + 1] = put_f<T>(a * r.y + b * r.x);
             }
         }
-        *reinterpret_cast<V*>(dst + e0) = lo;
-        if (two) *reinterpret_cast<V*>(dst + e1) = hi;
+        dst += ADJ && VE == 1 ? 2 * c : c * VE;
+        *reinterpret_cast<V*>(dst) = lo;
+        if (TWO) *reinterpret_cast<V*>(dst + (ADJ ? 1 : p.n_freq)) = hi;
         j += rows;
-        h += rows;
-        while (h >= heads) {
+        tk += step_t;
+        h += step_h;
+        if (h >= heads) {
             h -= heads;
             ++tk;
         }
@@ -153,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
             j = first;
             tk = first / heads;
             h = first - tk * heads;
-            live = c < g.head_chunks;
+            live = c < g.rot_chunks;
         }
         if (live) load();
     }
@@ -165,8 +174,11 @@ void launch(cudaStream_t s, const RopeParams& p) {
     const long long all = p.batch * p.tokens;
     const int heads = p.t[0].heads + p.t[1].heads;
     RopeGrid g;
-    g.head_chunks = p.n_freq / PAIRS + (p.dim - 2 * p.n_freq) / VE;
-    g.cols = g.head_chunks < kThreads ? g.head_chunks : kThreads;
+    g.rot_chunks = p.n_freq / PAIRS;
+    // turned in place, the tail is where it belongs
+    const bool in_place = (p.t[0].heads == 0 || p.t[0].x == p.t[0].out) && (p.t[1].heads == 0 || p.t[1].x == p.t[1].out);
+    g.tail_chunks = in_place ? 0 : (p.dim - 2 * p.n_freq) / VE;
+    g.cols = g.rot_chunks < kThreads ? g.rot_chunks : kThreads;
     // Tokens a block: a block costs its accesses a thread and some for its start (98,304 tokens of 32
     // heads of 64, with 2, 4, 8 and 16 accesses: 148, 135, 130, 134 us); while there are few blocks, the
     // last round of them over the SMs counts whole.  With few tokens the heads are split over blocks, and
@@ -193,6 +205,7 @@ void launch(cudaStream_t s, const RopeParams& p) {
         // at least one access for every thread
         if (g.heads_per_block < rows) g.heads_per_block = rows < heads ? rows : heads;
     }
+    if (g.heads_per_block > kMaxHeads) g.heads_per_block = kMaxHeads;
     g.head_blocks = (heads + g.heads_per_block - 1) / g.heads_per_block;
     const long long grid = token_blocks * g.head_blocks;
     M3R_REQUIRE(grid <= 0x7FFFFFFFLL, "rope: too many tokens for one call");
