@@ -599,6 +599,24 @@ void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, 
 long long padded_k(int k) { return (static_cast<long long>(k) + 15) / 16 * 16; }
 size_t round256(size_t b) { return (b + 255) / 256 * 256; }
 
+// Time of a tile shape, from what the shapes measured alone: a start (with the last epilogue), and for
+// every round of tiles over the SMs its k-blocks, each as long as the larger of the tile's own rate and
+// the 12 TB/s at which all SMs together read L2, or its epilogue.  (us: 1,536 x 1,024 x 1,024 8.7, 6.6
+// and 8.9 with tiles of 256 x 256, 128 x 128 and 128 x 64; 1,536 x 3,072 x 1,024 9.2, 9.8, 14.6; 300 x
+// 4,096 x 4,096 16.1, 14.2, 23.4; 200 x 1,024 x 1,024 8.4, 6.3, 6.0.)
+double tile_us(int bn, int cg, long long rows, int n, int k, int sms) {
+    const double start = bn == 256 ? 6.3 : bn == 128 ? 4.2 : 4.0;
+    const double block = bn == 256 ? 0.298 : bn == 128 ? 0.303 : 0.25;
+    const double epilogue = bn == 256 ? 3.9 : bn == 128 ? 2.2 : 1.4;
+    const long long tiles = static_cast<long long>(cdiv(rows, 128 * cg)) * cdiv(n, bn);
+    const long long units = sms / cg;
+    const long long rounds = (tiles + units - 1) / units;
+    const double busy = static_cast<double>(tiles < units ? tiles : units) * cg;
+    const double fabric = busy * (128 + bn / cg) * 128 / 12e6;  // us a k-block at 12 TB/s
+    const double round = cdiv(k, 128) * (block > fabric ? block : fabric);
+    return start + round + (rounds - 1) * (round > epilogue ? round : epilogue);
+}
+
 // One or two rows that fit the default shared memory of a block, and up to 4 short ones, take the
 // one-launch kernel (device time with n = 4,096: 4 rows of 1,024 5.3 us against 6.3 in the other, 4 of
 // 4,096 8.8 against 7.9; 8 of 1,024 9.2 against 5.6).
@@ -676,10 +694,11 @@ void int8_linear(cudaStream_t s, const Int8LinearParams& p) {
     if (p.rows <= 32) return launch_skinny<32>(s, p, xq, ldq, xs, sms);
     if (p.rows <= 64) return launch_skinny<64>(s, p, xq, ldq, xs, sms);
     if (p.rows <= 128) return launch_skinny<128>(s, p, xq, ldq, xs, sms);
-    // the largest tile that gives every SM one
-    if (static_cast<long long>(cdiv(p.rows, 256)) * cdiv(p.n, 256) * 2 >= sms)
+    const double big = tile_us(256, 2, p.rows, p.n, p.k, sms), mid = tile_us(128, 1, p.rows, p.n, p.k, sms),
+                 low = tile_us(64, 1, p.rows, p.n, p.k, sms);
+    if (big <= mid && big <= low)
         launch<256, 2>(s, p, xq, ldq, xs, sms);
-    else if (static_cast<long long>(cdiv(p.rows, 128)) * cdiv(p.n, 128) >= sms)
+    else if (mid <= low)
         launch<128, 1>(s, p, xq, ldq, xs, sms);
     else
         launch<64, 1>(s, p, xq, ldq, xs, sms);

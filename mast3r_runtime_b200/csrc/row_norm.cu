@@ -394,16 +394,16 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
 // Rows to threads.  Short rows share a warp, 8 values a lane.  With many rows, a warp each up to
 // 1,024 values (98,304 rows of 1,024, 32-bit stream: 199 us, against 226 with a block each); with
 // few, a block each, 8 values a thread, so that a row's chain of loads and reductions is short
-// (1,536 rows of 1,024 quantised: 4.0 us against 6.8).
+// (1,536 rows of 1,024 quantised: 4.0 us against 6.8; 6,144 rows of 1,024, whole operator: 18.5
+// against 20.4, 24,576: 57.8 against 55.4; 6,144 rows of 512: 9.7 either way; 12,288 of 1,024
+// quantised: 11 against 7 with a warp each).
 void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
     if (p.cols <= 32) return launch<true, 1, 4>(s, p, 128);
     if (p.cols <= 64) return launch<true, 1, 8>(s, p, 128);
     if (p.cols <= 128) return launch<true, 1, 16>(s, p, 128);
     if (p.cols <= 256) return launch<true, 1, 32>(s, p, 128);
-    if (p.rows > 148 * 16) {
-        if (p.cols <= 512) return launch<true, 2, 32>(s, p, 128);
-        if (p.cols <= 1024) return launch<true, 4, 32>(s, p, 128);
-    }
+    if (p.cols <= 512 && p.rows > 148 * 16) return launch<true, 2, 32>(s, p, 128);
+    if (p.cols <= 1024 && p.rows > 148 * (is_quantize(p) ? 16 : 96)) return launch<true, 4, 32>(s, p, 128);
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
     if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, 0>(s, p, threads(1));
     const int blocks = 148 * (1024 / threads(2));  // at 64 registers
