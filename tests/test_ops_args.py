@@ -64,7 +64,7 @@ def test_c_refusals():
         refused("m3r_quantize_rows", quantize(**bad), text)
     refused("m3r_quantize_rows", None, "null")
 
-    def linear(xt=1, ot=1, act=0, m=4, n=32, k=64, ldx=64, ldw=64, ldo=32, x=256, xs=0, w=256, ws=256, b=0, o=256,
+    def linear(xt=1, ot=1, act=0, m=400, n=32, k=64, ldx=64, ldw=64, ldo=32, x=256, xs=0, w=256, ws=256, b=0, o=256,
                work=256, size=1 << 20):
         return LINEAR.pack(0, xt, ot, act, m, n, k, ldx, ldw, ldo, x, xs, w, ws, b, o, work, size, 0)
 
