@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -57,6 +58,14 @@ int64_t device_of(const char* op, std::initializer_list<const Tensor*> all) {
         if (grad && t->requires_grad()) fail(op, "no gradient is computed (use torch.no_grad() or detach the tensors)");
     }
     return dev;
+}
+
+// A tensor that a call writes over: its version counts, and no element is there twice.
+void check_written(const char* op, const char* name, const Tensor& t) {
+    if (t.is_inference() && !c10::InferenceMode::is_enabled())
+        fail(op, std::string(name) + " is an inference tensor and can be written in inference mode only");
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.stride(i) == 0 && t.size(i) > 1) fail(op, std::string(name) + " has elements that share memory");
 }
 
 int float_code(const char* op, const char* name, at::ScalarType t) {
@@ -325,6 +334,7 @@ PyObject* residual_norm(PyObject* const* a) {
     p.eps = static_cast<float>(number_arg(op, "eps", a[10]));
     const at::ScalarType out_type = dtype_arg(op, a[11], (y.defined() ? y : x).scalar_type());
     const bool inplace = bool_arg(a[12]);
+    if (inplace) check_written(op, "x", x);
     const Tensor res = inplace ? x : empty(x.sizes(), x.scalar_type(), dev);
     p.ldr = inplace ? r.ld : r.cols;
     Tensor out, scale;
@@ -398,6 +408,10 @@ PyObject* rope(PyObject* const* a) {
     } else {
         oq = empty(q.sizes(), q.scalar_type(), dev);
         if (k.defined()) ok = empty(k.sizes(), k.scalar_type(), dev);
+    }
+    if (inplace || oq0.defined()) {
+        check_written(op, "q's result", oq);
+        if (ok.defined()) check_written(op, "k's result", ok);
     }
     rope_tensor(op, "q", q, oq, q, p.t[0]);
     if (k.defined()) rope_tensor(op, "k", k, ok, q, p.t[1]);

@@ -157,7 +157,8 @@ def linear64(q, s, w, ws, bias, act, out_dtype):
 
 SHAPES = [(1, 1, 1), (1, 5, 16), (1, 4096, 1024), (2, 130, 257), (3, 1153, 1000), (7, 64, 4096), (8, 1000, 33),
           (9, 300, 512), (16, 4096, 640), (17, 129, 2048), (24, 2048, 4096), (33, 520, 128), (64, 1000, 999),
-          (65, 96, 384), (128, 1152, 384), (129, 257, 129), (577, 1153, 1000), (1536, 2304, 768), (2500, 4100, 1040)]
+          (65, 96, 384), (128, 1152, 384), (129, 257, 129), (577, 1153, 1000), (1536, 2304, 768), (2500, 4100, 1040),
+          (20000, 1040, 768), (19500, 1501, 1000), (26001, 600, 70)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -499,3 +500,180 @@ def test_same_inputs_give_the_same_bits(ops):
     first = block_entry(ops, s)
     for _ in range(5):
         assert all(torch.equal(i, j) for i, j in zip(first, block_entry(ops, s)))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 24, 100, 600, 20000])
+def test_linear_captured_with_its_quantisation(ops, rows):
+    """The product starts while the quantisation still runs; captured, replayed on new inputs and
+    mixed with calls outside the graph, the results stay those of one call at a time."""
+    k, n = 1000, 520
+    x = rnd(rows, k, seed=rows, dtype=torch.bfloat16)
+    wq, ws = ops.quantize_weight(rnd(n, k, seed=2, scale=k ** -0.5))
+    b = rnd(n, seed=3)
+    ops.int8_linear(x, wq, ws, b)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        first = ops.int8_linear(x, wq, ws, b, act="gelu")
+        second = ops.int8_linear(x * 0.5, wq, ws, b)
+    for seed in (7, 8):
+        x.copy_(rnd(rows, k, seed=seed, dtype=torch.bfloat16))
+        g.replay()
+        mixed = ops.int8_linear(x, wq, ws, b, act="gelu")
+        torch.cuda.synchronize()
+        want = ops.int8_linear(x, wq, ws, b, act="gelu")
+        half_x = ops.int8_linear(x * 0.5, wq, ws, b)
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(mixed, want) and torch.equal(second, half_x)
+        q, s = levels(x)
+        ref, tol = linear64(q, s, wq, ws, b, "gelu", torch.bfloat16)
+        close(want, ref, tol)
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing has to be set up before a capture."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    code = (
+        "import torch\n"
+        "from mast3r_runtime_b200 import ops\n"
+        "x = torch.randn(300, 256, device='cuda').half(); w = torch.randn(128, 256, device='cuda')\n"
+        "f, _ = ops.rope_frequencies(64); pos = torch.arange(300, device='cuda')\n"
+        "torch.cuda.synchronize()\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    wq, ws = ops.quantize_weight(w)\n"
+        "    r, h = ops.residual_norm(x, x, None)\n"
+        "    y = ops.int8_linear(h, wq, ws)\n"
+        "    q, _ = ops.rope(y.view(300, 2, 64), None, pos, f)\n"
+        "    z = ops.int8_linear(x[:1], wq, ws); t = ops.int8_linear(x[:20], wq, ws)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "r2, h2 = ops.residual_norm(x, x, None)\n"
+        "y2 = ops.int8_linear(h2, *ops.quantize_weight(w))\n"
+        "assert torch.equal(y, y2) and torch.equal(q, ops.rope(y2.view(300, 2, 64), None, pos, f)[0])\n"
+        "assert torch.equal(z, ops.int8_linear(x[:1], wq, ws)) and torch.equal(t, ops.int8_linear(x[:20], wq, ws))\n"
+        "print('fine')\n")
+    out = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "fine" in out.stdout, out.stderr[-2000:]
+
+
+def test_threads(ops):
+    """Calls from several threads at once, each on its own stream."""
+    import threading
+
+    states = [block_state(ops, 100 + i) for i in range(4)]
+    want = [block_entry(ops, s) for s in states]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = block_entry(ops, states[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.skipif("torch.cuda.device_count() < 2")
+def test_another_device_than_the_current_one(ops):
+    s = {k: v.to("cuda:1") if torch.is_tensor(v) else v for k, v in block_state(ops, 71).items()}
+    want = block_entry(ops, block_state(ops, 71))
+    got = block_entry(ops, s)
+    assert torch.cuda.current_device() == 0
+    for a, b in zip(got, want):
+        assert a.device.index == 1 and torch.equal(a.cpu(), b.cpu())
+    with pytest.raises(ValueError, match="different devices"):
+        ops.residual_norm(s["x"], want[0].half(), None)
+
+
+def test_more_than_2_to_the_31_elements(ops):
+    """Offsets past 32 bits: the last rows and tokens of tensors of over 2^31 elements."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free device memory")
+    tokens, heads = 1_100_000, 16
+    x = torch.zeros(tokens, heads, 128, dtype=torch.bfloat16, device="cuda")
+    x[-2:] = rnd(2, heads, 128, seed=1, dtype=torch.bfloat16)
+    pos = torch.arange(tokens, device="cuda")
+    f, _ = ops.rope_frequencies(128)
+    o, _ = ops.rope(x, None, pos, f)
+    want, tol = rope64(x[None, -2:], pos[None, None, -2:], f, 1.0, False, 1)
+    close(o[None, -2:], want, tol)
+    planes = torch.zeros(heads, tokens, 128, dtype=torch.bfloat16, device="cuda")
+    ops.rope(x, None, pos, f, out=(planes.transpose(0, 1), None))
+    assert torch.equal(planes[:, -2:].transpose(0, 1), o[-2:])
+    del planes, o
+    rows = x.view(-1, 2048)
+    r, h = ops.residual_norm(rows, rows, None, norm="rms")
+    r2, h2 = ops.residual_norm(rows[-2:].clone(), rows[-2:].clone(), None, norm="rms")
+    # two rows are a block each, many are copied ahead: the sums' order is the same
+    assert torch.equal(r[-2:], r2)
+    close(h[-2:], h2.double(), 2 * half(h.dtype) * h2.double().abs() + 1e-6)
+    del r, h, x, rows
+    q = torch.ones(600_000, 64, dtype=torch.int8, device="cuda")
+    w = ints(4096, 64, 3)
+    y = ops.int8_linear(q, w, torch.ones(4096, device="cuda"), x_scale=torch.ones(600_000, device="cuda"))
+    assert torch.equal(y[-1].float(), w.float().sum(1).bfloat16().float()) and torch.equal(y[-1], y[0])
+
+
+def test_refusals_on_the_device(ops):
+    x = rnd(4, 32, seed=1)
+    wq, ws = ops.quantize_weight(rnd(8, 32, seed=2))
+    f, _ = ops.rope_frequencies(32)
+    q, pos = x.view(4, 1, 32), torch.arange(4, device="cuda")
+    for call, text in (
+            (lambda: ops.quantize_rows(x.double()), "bfloat16, float16 or float32"),
+            (lambda: ops.quantize_rows(x.t()), "contiguous"),
+            (lambda: ops.quantize_rows(x[0, 0]), "dimension"),
+            (lambda: ops.int8_linear(x, wq.float(), ws), "int8"),
+            (lambda: ops.int8_linear(x[:, :16], wq, ws), "weight must be"),
+            (lambda: ops.int8_linear(x, wq, ws[:4]), "weight_scale"),
+            (lambda: ops.int8_linear(x, wq, ws, ws.half()), "bias"),
+            (lambda: ops.int8_linear(x, wq, ws, act="tanh"), "activation"),
+            (lambda: ops.int8_linear(x, wq, ws, out_dtype=torch.float64), "out_dtype"),
+            (lambda: ops.int8_linear(x, wq, ws, x_scale=ws), "x_scale"),
+            (lambda: ops.int8_linear(x.to(torch.int8), wq, ws), "x_scale"),
+            (lambda: ops.int8_linear(rnd(4, 24).to(torch.int8)[:, 4:], wq[:, :20], ws, x_scale=ws[:4]), "16-byte"),
+            (lambda: ops.int8_linear(x[:, 1:], wq[:, 1:], ws), "16-byte"),
+            (lambda: ops.int8_linear(x, wq.cpu(), ws), "CUDA|device"),
+            (lambda: ops.residual_norm(x, x[:2], None), "shape"),
+            (lambda: ops.residual_norm(x, x, ws), "weight"),
+            (lambda: ops.residual_norm(x, x, None, norm="batch"), "norm"),
+            (lambda: ops.residual_norm(x, None, None, post_norm="rms"), "without y"),
+            (lambda: ops.residual_norm(x, x, None, gate=x[:3]), "gate"),
+            (lambda: ops.residual_norm(x, x, None, eps=float("nan")), "eps"),
+            (lambda: ops.residual_norm(x[:1].expand(4, 32), x, None), "overlap"),
+            (lambda: ops.rope(q, None, pos.float(), f), "positions"),
+            (lambda: ops.rope(q, None, pos[:3], f), "positions"),
+            (lambda: ops.rope(q, q.half(), pos, f), "type"),
+            (lambda: ops.rope(q, q[:2], pos, f), "k must be"),
+            (lambda: ops.rope(q, None, pos, ops.rope_frequencies(64)[0]), "frequencies"),
+            (lambda: ops.rope(q, None, pos, f, inplace=True, out=(q, None)), "exclude"),
+            (lambda: ops.rope(q, None, pos, f, out=(q.half(), None)), "match"),
+            (lambda: ops.rope(q[:, :, :1].expand(4, 1, 32), None, pos, f), "contiguous"),
+            (lambda: ops.rope(q.expand(4, 3, 32), None, pos, f, inplace=True), "share memory"),
+            (lambda: ops.residual_norm(x.clone().requires_grad_(), x, None), "gradient")):
+        with pytest.raises(ValueError, match=text):
+            call()
+    with torch.no_grad():
+        ops.residual_norm(x.clone().requires_grad_(), x, None)
+    with torch.inference_mode():
+        y = x + 1
+        ops.residual_norm(y, x, None, inplace=True)
+    with pytest.raises(ValueError, match="inference"):
+        ops.residual_norm(y, x, None, inplace=True)
+    # an in-place call counts as a change of the tensor
+    z = x.clone()
+    v = z._version
+    ops.residual_norm(z, x, None, inplace=True)
+    assert z._version == v + 1
+    ops.status(0)
