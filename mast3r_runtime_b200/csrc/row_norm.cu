@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH ==
 
 // Many long rows: a block keeps its next rows of x and y on their way into shared memory with bulk
 // copies, so that the loads do not wait for the reductions of the row before and take no registers
-// (24,576 rows of 4,096, bf16: 140 us against 192; quantising alone gains nothing, 71 against 65).
+// (24,576 rows of 4,096, bf16: 132 us against 192; quantising alone gains nothing, 71 against 65).
 constexpr int kStreamStages = 4;
 
 __global__ void __launch_bounds__(1024) row_stream_kernel(const __grid_constant__ RowNormParams p, int stages) {
@@ -374,17 +374,22 @@ void launch(cudaStream_t s, const RowNormParams& p, int threads) {
     M3R_CUDA(cudaGetLastError());
 }
 
-void launch_stream(cudaStream_t s, const RowNormParams& p, int threads) {
-    // all of an SM's registers (64 a thread) and shared memory, in as many blocks as that makes
-    constexpr int kMost = 225 * 1024;
+// All of an SM's registers (64 a thread) in as many blocks as that makes, and shared memory but for
+// some that is left to L1, where the weight and gate vectors of every row come from (24,576 rows of
+// 4,096, bf16, with 225, 180 and 140 KB of rings: 140, 132, 133 us; 50,000 of 2,048: 145, 138, 148).
+// False where a block's share does not hold a row.
+bool launch_stream(cudaStream_t s, const RowNormParams& p, int threads) {
+    constexpr int kMost = 180 * 1024;
     const int per_sm = 1024 / threads;
     const int row = p.cols * (op_size(p.x_dt) + (p.y != nullptr ? op_size(p.y_dt) : 0));
-    const int room = kMost / per_sm - (per_sm > 1 ? 2048 : 0);
+    const int room = kMost / per_sm - 2048;
     const int stages = room / row < kStreamStages ? room / row : kStreamStages;
+    if (stages < 1) return false;
     static unsigned done = 0;
     allow_smem(row_stream_kernel, kMost, done);
     row_stream_kernel<<<148 * per_sm, threads, stages * row, s>>>(p, stages);
     M3R_CUDA(cudaGetLastError());
+    return true;
 }
 
 bool aligned(const void* p, long long ld, int dt, int bytes) {
@@ -407,7 +412,7 @@ void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
     if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, 0>(s, p, threads(1));
     const int blocks = 148 * (1024 / threads(2));  // at 64 registers
-    if (p.rows >= 2LL * blocks && !is_quantize(p)) return launch_stream(s, p, threads(2));
+    if (p.rows >= 2LL * blocks && !is_quantize(p) && launch_stream(s, p, threads(2))) return;
     launch<true, 2, 0>(s, p, threads(2));
 }
 
