@@ -456,9 +456,12 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---------------------------------------------------------------- dependent launches
-// A kernel launched as a programmatic dependent of the one before it on the stream starts once
-// every block of that one has called grid_dependency_start (or left), and sees its results after
-// grid_dependency_wait.  Both do nothing in ordinary launches.
+// A kernel launched as a programmatic dependent of the one before it on the stream may start once
+// every block of that one has called grid_dependency_start or left.  grid_dependency_wait returns when
+// that kernel has finished and its results can be seen -- and then everything before it has, as long as
+// it waited too.  A kernel launched so touches no memory before it has waited, calls
+// grid_dependency_start only after, and loads with plain loads (no __ldg): what the kernel before writes
+// is not constant while it runs.  Both do nothing in ordinary launches.
 __device__ __forceinline__ void grid_dependency_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

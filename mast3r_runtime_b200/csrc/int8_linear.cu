@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    grid_dependency_wait();  // rows quantised by the kernel before
+    grid_dependency_wait();
     const uint32_t full_c = CG == 2 ? cluster_addr(smem_u32(full), 0) : smem_u32(full);
     const uint32_t tempty_c = CG == 2 ? cluster_addr(smem_u32(tempty), 0) : smem_u32(tempty);
     const uint32_t peer_abort_c =
@@ -442,12 +442,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                            : (grp + (j >> 6) * kEpiGroups) * 64 + (j & 63));
                 float4 q = make_float4(0, 0, 0, 0);
                 if (c < p.N) {
-                    q.x = __ldg(p.ws + c);
-                    if (p.bias) q.z = __ldg(p.bias + c);
+                    q.x = p.ws[c];
+                    if (p.bias) q.z = p.bias[c];
                 }
                 if (c + 1 < p.N) {
-                    q.y = __ldg(p.ws + c + 1);
-                    if (p.bias) q.w = __ldg(p.bias + c + 1);
+                    q.y = p.ws[c + 1];
+                    if (p.bias) q.w = p.bias[c + 1];
                 }
                 cols[j >> 1] = q;
             }
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const long long r = row0 + 8 * i + (lane >> 2);
-                xs[i] = r < p.M ? __ldg(p.xs + r) : 0.0f;
+                xs[i] = r < p.M ? p.xs[r] : 0.0f;
             }
             if (!mbar_wait(&tfull[buf], (tcount >> 1) & 1, abort_flag, kDevTimeoutEpilogue, err)) {
                 abort_pair();
@@ -517,18 +517,6 @@ int sm_count() {
     return n;
 }
 
-// Cluster size, and after the rows' quantisation (a kernel of this call) a dependent launch: the
-// product sets up its barriers and TMEM, and fetches its first weights, while that one runs.
-int launch_attributes(cudaLaunchAttribute (&attr)[2], int cluster, const Int8LinearParams& q) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    return q.x_dt == OP_I8 ? 1 : 2;
-}
-
 template <int BN, int CG>
 void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long long ldq, const float* xs, int sms) {
     using C = I8Cfg<BN, CG>;
@@ -557,15 +545,8 @@ void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long lo
                                 : tmap_2d(q.out_dt, q.out, q.rows, q.n, q.ldo, 32);
     const int units = p.tiles_m * p.tiles_n;
     const int max_units = sms / CG;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CG * (units < max_units ? units : max_units));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = C::SMEM_BYTES;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, CG, q);
-    M3R_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, p));
+    const LaunchConfig c(CG * (units < max_units ? units : max_units), kThreads, C::SMEM_BYTES, s, CG);
+    M3R_CUDA(cudaLaunchKernelEx(&c.cfg, kern, ma, mb, mc, p));
 }
 
 template <int NT>
@@ -592,15 +573,9 @@ void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, 
     while (p.split < 8 && tiles * p.split * 2 <= 2 * sms && p.num_kb >= p.split * 4) p.split *= 2;
     const CUtensorMap mw = tmap_2d_u8(q.w, q.n, q.k, q.ldw, 128);
     const CUtensorMap mx = tmap_2d_u8(xq, q.rows, q.k, ldq, NT);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles) * p.split);
-    cfg.blockDim = dim3(kSkinnyThreads);
-    cfg.dynamicSmemBytes = C::SMEM_BYTES;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
-    cfg.numAttrs = launch_attributes(attr, p.split, q);
-    M3R_CUDA(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
+    p.early_w = q.x_dt != OP_I8;
+    const LaunchConfig c(static_cast<unsigned>(tiles) * p.split, kSkinnyThreads, C::SMEM_BYTES, s, p.split);
+    M3R_CUDA(cudaLaunchKernelEx(&c.cfg, kern, mw, mx, p));
 }
 
 long long padded_k(int k) { return (static_cast<long long>(k) + 15) / 16 * 16; }
@@ -651,8 +626,8 @@ void launch_gemv(cudaStream_t s, const Int8LinearParams& q, int sms) {
     p.out = q.out;
     const int blocks = cdiv(q.n, kGemvCols * (kGemvThreads / 32));
     const int most = 2 * sms;
-    int8_gemv_kernel<MR><<<blocks < most ? blocks : most, kGemvThreads, MR * p.kpad, s>>>(p);
-    M3R_CUDA(cudaGetLastError());
+    const LaunchConfig c(blocks < most ? blocks : most, kGemvThreads, MR * p.kpad, s);
+    M3R_CUDA(cudaLaunchKernelEx(&c.cfg, int8_gemv_kernel<MR>, p));
 }
 
 }  // namespace

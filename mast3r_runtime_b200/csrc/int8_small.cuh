@@ -63,11 +63,11 @@ template <class T>
 __device__ __forceinline__ void gemv_load8(const T* row, int e, int K, bool vec, float (&v)[8]) {
     if (vec && e + 8 <= K) {
         if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(row + e));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(row + e) + 1);
+            const float4 a = *reinterpret_cast<const float4*>(row + e);
+            const float4 b = reinterpret_cast<const float4*>(row + e)[1];
             v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
         } else {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + e));
+            const uint4 u = *reinterpret_cast<const uint4*>(row + e);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -140,19 +140,20 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
         for (int i = 0; i < kGemvCols; ++i) {
             const uint4* row = reinterpret_cast<const uint4*>(channel(i));
 #pragma unroll
-            for (int s = 0; s < 2; ++s) w[i][s] = c + 32 * s < chunks ? __ldg(row + c + 32 * s) : make_uint4(0, 0, 0, 0);
+            for (int s = 0; s < 2; ++s) w[i][s] = c + 32 * s < chunks ? row[c + 32 * s] : make_uint4(0, 0, 0, 0);
         }
     };
+    grid_dependency_wait();
     if (n0 < p.N) load(lane);
     if (p.x_dt == OP_I8) {
         for (int m = 0; m < MR; ++m) {
             const int8_t* row = static_cast<const int8_t*>(p.x) + m * p.ldx;
             for (int c = tid; c < chunks; c += kGemvThreads)
                 reinterpret_cast<uint4*>(sx + m * p.kpad)[c] =
-                    m < p.M ? __ldg(reinterpret_cast<const uint4*>(row) + c) : make_uint4(0, 0, 0, 0);
+                    m < p.M ? reinterpret_cast<const uint4*>(row)[c] : make_uint4(0, 0, 0, 0);
             if (tid < tail) sx[m * p.kpad + chunks * 16 + tid] = m < p.M ? static_cast<uint8_t>(row[chunks * 16 + tid]) : 0;
         }
-        if (tid < MR) scale[tid] = tid < p.M ? __ldg(p.x_scale + tid) : 0.0f;
+        if (tid < MR) scale[tid] = tid < p.M ? p.x_scale[tid] : 0.0f;
     } else if (p.x_dt == OP_F32) {
         gemv_quantise<float, MR>(p, sx, scale, part);
     } else if (p.x_dt == OP_F16) {
@@ -217,9 +218,9 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
             }
         const int n = first + lane / MR, m = lane % MR;
         if (lane < kGemvCols * MR && n < p.N && m < p.M) {
-            const float b = p.bias ? __ldg(p.bias + n) : 0.0f;
+            const float b = p.bias ? p.bias[n] : 0.0f;
             store1(p.out, p.out_dt, m * p.ldo + n,
-                   finish1(mine, scale[m], __ldg(p.ws + n), b, p.act, p.out_dt == OP_F32));
+                   finish1(mine, scale[m], p.ws[n], b, p.act, p.out_dt == OP_F32));
         }
     }
 }
@@ -231,6 +232,7 @@ struct SkinnyParams {
     const float* ws;
     const float* bias;
     int act, out_dt, out_vec;  // out_vec: 4 values of a row are an aligned access
+    int early_w;               // the kernel before is the quantisation of this call
     void* out;
     long long ldo;
 };
@@ -302,7 +304,9 @@ __global__ void __launch_bounds__(kSkinnyThreads)
 
     if (tid == 0) {
         // ------------------------------------------------ TMA producer
-        // the first weights travel while the kernel before (the rows' quantisation) still runs
+        // the first weights travel while this call's quantisation still runs: it has waited for all that
+        // came before
+        if (!p.early_w) grid_dependency_wait();
         const int early = min(STAGES, kb1 - kb0);
         for (int s = 0; s < early; ++s) {
             mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
@@ -346,19 +350,19 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     }
     __syncwarp();
     // ------------------------------------------------ sums to shared memory: part[token][channel]
+    grid_dependency_wait();
     const int lane = tid & 31;
     float ws[4], bias[4];  // of the 4 channels that this thread finishes
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const int n = n0 + 4 * lane + c;
-        ws[c] = n < p.N ? __ldg(p.ws + n) : 0.0f;
-        bias[c] = n < p.N && p.bias ? __ldg(p.bias + n) : 0.0f;
+        ws[c] = n < p.N ? p.ws[n] : 0.0f;
+        bias[c] = n < p.N && p.bias ? p.bias[n] : 0.0f;
     }
     {
         volatile int dummy = 0;
         mbar_wait(done, 0, &dummy, kDevTimeoutEpilogue, err);
     }
-    grid_dependency_wait();  // the rows' scales
     tc_fence_after();
     __syncthreads();  // every load has landed and been multiplied: the stages' memory is free
     int* part = reinterpret_cast<int*>(smem);
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             int sum[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int r = 0; r < 8; ++r) sum[0] += v[u][r].x, sum[1] += v[u][r].y, sum[2] += v[u][r].z, sum[3] += v[u][r].w;
-            const float xs = __ldg(p.xs + t);
+            const float xs = p.xs[t];
             float y[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) y[c] = finish1(sum[c], xs, ws[c], bias[c], p.act, p.out_dt == OP_F32);

@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "launch.h"
 #include "ops.h"
 #include "tmap.h"
 
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rope_kernel(const __gr
     const int split = p.t[0].heads - head0;  // the block's heads from here on are the second tensor's
     const int ntok = min(g.tokens_per_block, all - tok0);
     const int tid = threadIdx.x;
+    grid_dependency_wait();
     if (tid < 2 * ntok) {
         const int tk = tid >> 1, axis = tid & 1;
         const int b = (tok0 + tk) / static_cast<int>(p.tokens), t = tok0 + tk - b * static_cast<int>(p.tokens);
@@ -209,8 +211,8 @@ void launch(cudaStream_t s, const RopeParams& p) {
     g.head_blocks = (heads + g.heads_per_block - 1) / g.heads_per_block;
     const long long grid = token_blocks * g.head_blocks;
     M3R_REQUIRE(grid <= 0x7FFFFFFFLL, "rope: too many tokens for one call");
-    rope_kernel<T, VE, ADJ><<<static_cast<unsigned>(grid), kThreads, 0, s>>>(p, g);
-    M3R_CUDA(cudaGetLastError());
+    const LaunchConfig c(static_cast<unsigned>(grid), kThreads, 0, s);
+    M3R_CUDA(cudaLaunchKernelEx(&c.cfg, rope_kernel<T, VE, ADJ>, p, g));
 }
 
 // Largest vector that the layout, the alignment and every stride allow.

@@ -7,6 +7,7 @@ value, U = 2^-24 one 32-bit rounding.  8-bit values and integer sums are compare
 from __future__ import annotations
 
 import math
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -527,6 +528,71 @@ def test_linear_captured_with_its_quantisation(ops, rows):
         q, s = levels(x)
         ref, tol = linear64(q, s, wq, ws, b, "gelu", torch.bfloat16)
         close(want, ref, tol)
+
+
+def test_calls_start_behind_what_they_read(ops):
+    """An operator may be launched before the kernel ahead of it has finished: inputs, weights and scales
+    written just before it, by torch or by another operator, on one stream or joined from another,
+    eagerly and in a graph, are the ones it reads; and what it writes over has been read."""
+    n, k, m = 512, 1024, 2048
+    big = rnd(4096, 4096, seed=1)
+    side = torch.cuda.Stream()
+    xs = [rnd(m, k, seed=10 + i, dtype=torch.bfloat16) for i in range(3)]
+    wt = [rnd(n, k, seed=20 + i, scale=k ** -0.5) for i in range(3)]
+    f, _ = ops.rope_frequencies(64)
+    pos = torch.arange(m, device="cuda")
+    x, w = torch.empty_like(xs[0]), torch.empty_like(wt[0])
+
+    def chain(ops, i, rows):
+        big @ big  # keeps the device busy, so that launches queue up
+        x.copy_(xs[i])
+        w.copy_(wt[i])
+        wq, ws = ops.quantize_weight(w)  # read by the next call
+        y = ops.int8_linear(x[:rows], wq, ws)
+        q, s = ops.quantize_rows(x)
+        wq2, ws2 = ops.quantize_weight(w * 2)
+        z = ops.int8_linear(q[:rows], wq2, ws2, x_scale=s[:rows], out_dtype=torch.bfloat16)
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            t = z * 3
+            r, h = ops.residual_norm(t, y, None)
+        main.wait_stream(side)
+        o, _ = ops.rope(h.view(rows, -1, 64), None, pos[:rows], f)
+        r2, h2 = ops.residual_norm(o.view(rows, n), z, None, inplace=True)
+        y.zero_()
+        return y, z, r, h, o, h2
+
+    def alone(fn):
+        """fn with the device idle before and after."""
+        def call(*a, **kw):
+            torch.cuda.synchronize()
+            r = fn(*a, **kw)
+            torch.cuda.synchronize()
+            return r
+
+        return call
+
+    slow = SimpleNamespace(**{name: alone(getattr(ops, name)) for name in ops.__all__})
+    for rows in (1, 4, 20, 200, m):
+        want = [[v.clone() for v in chain(slow, i, rows)] for i in range(3)]
+        for _ in range(3):
+            got = [chain(ops, i, rows) for i in range(3)]
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert all(torch.equal(u, v) for u, v in zip(a, b))
+        graphs = []
+        for i in range(3):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = chain(ops, i, rows)
+            graphs.append((g, out))
+        for _ in range(2):
+            for g, _ in graphs:
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, a), b in zip(graphs, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
 def test_first_calls_of_a_process_inside_a_capture():
