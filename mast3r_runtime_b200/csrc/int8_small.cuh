@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         // ------------------------------------------------ MMA issuer
         constexpr uint32_t idesc = idesc_i8kind(128, NT);
         int it = 0;
+        grid_dependency_wait();  // the limit of the waits below counts from here
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
             const int s = it % STAGES;
             if (!mbar_wait(&full[s], (it / STAGES) & 1, abort_flag, kDevTimeoutMma, err)) break;
