@@ -473,6 +473,13 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 
+// 1 / x, relative error 2^-23
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // GELU, tanh approximation (backends/python/vit_encoder.py:18-20).
 __device__ __forceinline__ float gelu_tanh(float x) {
     const float k0 = 0.7978845608028654f;  // sqrt(2 / pi)

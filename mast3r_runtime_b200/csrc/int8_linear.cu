@@ -118,7 +118,7 @@ __device__ __forceinline__ float tanh_approx(float x) {
 
 // x / 2 (1 + tanh u) = x / (1 + exp(-2 u)), to a few 32-bit roundings
 __device__ __forceinline__ float gelu_f32(float x, float u) {
-    return x * __frcp_rn(1.0f + ex2_approx(-2.885390081777927f * u));
+    return x * rcp_approx(1.0f + ex2_approx(-2.885390081777927f * u));
 }
 
 // Two neighbouring columns of a row: acc * xs * ws + bias, then the activation.
@@ -550,7 +550,8 @@ void launch(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long lo
 }
 
 template <int NT>
-void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long long ldq, const float* xs, int sms) {
+void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, long long ldq, const float* xs,
+                   int split) {
     using C = SkinnyCfg<NT>;
     auto kern = int8_skinny_kernel<NT>;
     static unsigned done = 0;
@@ -558,7 +559,9 @@ void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, 
     SkinnyParams p;
     p.M = static_cast<int>(q.rows);
     p.N = q.n;
+    p.tiles_n = cdiv(q.n, 128);
     p.num_kb = cdiv(q.k, 128);
+    p.split = split;
     p.xs = xs;
     p.ws = q.w_scale;
     p.bias = q.bias;
@@ -567,14 +570,11 @@ void launch_skinny(cudaStream_t s, const Int8LinearParams& q, const int8_t* xq, 
     p.out = q.out;
     p.ldo = q.ldo;
     p.out_vec = q.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(q.out) % (4 * op_size(q.out_dt)) == 0;
-    // k over as many CTAs as there is room for, two k-blocks each at least
-    const int tiles = cdiv(q.n, 128);
-    p.split = 1;
-    while (p.split < 8 && tiles * p.split * 2 <= 2 * sms && p.num_kb >= p.split * 4) p.split *= 2;
     const CUtensorMap mw = tmap_2d_u8(q.w, q.n, q.k, q.ldw, 128);
     const CUtensorMap mx = tmap_2d_u8(xq, q.rows, q.k, ldq, NT);
     p.early_w = q.x_dt != OP_I8;
-    const LaunchConfig c(static_cast<unsigned>(tiles) * p.split, kSkinnyThreads, C::SMEM_BYTES, s, p.split);
+    const int tiles = p.tiles_n * cdiv(q.rows, NT);
+    const LaunchConfig c(static_cast<unsigned>(tiles) * split, kSkinnyThreads, C::SMEM_BYTES, s, split);
     M3R_CUDA(cudaLaunchKernelEx(&c.cfg, kern, mw, mx, p));
 }
 
@@ -597,6 +597,31 @@ double tile_us(int bn, int cg, long long rows, int n, int k, int sms) {
     const double fabric = busy * (128 + bn / cg) * 128 / 12e6;  // us a k-block at 12 TB/s
     const double round = cdiv(k, 128) * (block > fabric ? block : fabric);
     return start + round + (rounds - 1) * (round > epilogue ? round : epilogue);
+}
+
+// The same for the kernel that splits k over clusters of `split` CTAs, with the split that takes least: its
+// start, the k-blocks of an SM, the tokens that a CTA joins, 8 at a time, and 3 us for every two CTAs more
+// than the two that an SM holds.  (us, 8-bit rows: 24 x 4,096 x 4,096 7.5, 64 x 1,024 x 4,096 6.9,
+// 100 x 1,153 x 1,000 7.1, 128 x 4,096 x 4,096 12.3, 300 x 1,024 x 4,096 10.9 against 12.9 in tiles of 64
+// columns, 1,024 x 256 x 8,192 12.0 against 22.3, 300 x 4,096 x 4,096 29 against 13.5.)
+double skinny_us(long long rows, int n, int k, int sms, int& nt, int& split) {
+    nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    const double start = nt <= 32 ? 3.8 : 4.8;
+    const double block = nt == 16 ? 0.25 : nt == 32 ? 0.27 : nt == 64 ? 0.45 : 0.6;
+    const long long tiles = static_cast<long long>(cdiv(rows, nt)) * cdiv(n, 128);
+    const int num_kb = cdiv(k, 128), tokens = rows < nt ? static_cast<int>(rows) : nt;
+    double best = 0;
+    split = 0;
+    for (int sp = 1; sp <= 8 && sp <= num_kb; sp *= 2) {
+        const long long rounds = (tiles * sp + sms - 1) / sms;
+        const double us = start + (rounds - 1) / 2 * 3.0 + static_cast<double>(rounds) * cdiv(num_kb, sp) * block +
+                          0.8 * cdiv(tokens, 8 * sp);
+        if (split == 0 || us < best) {
+            best = us;
+            split = sp;
+        }
+    }
+    return best;
 }
 
 // One or two rows that fit the default shared memory of a block, and up to 4 short ones, take the
@@ -669,14 +694,22 @@ void int8_linear(cudaStream_t s, const Int8LinearParams& p) {
         ldq = padded_k(p.k);
         xs = sc;
     }
-    // few rows: the weights' bytes are the work
-    if (p.rows <= 16) return launch_skinny<16>(s, p, xq, ldq, xs, sms);
-    if (p.rows <= 32) return launch_skinny<32>(s, p, xq, ldq, xs, sms);
-    if (p.rows <= 64) return launch_skinny<64>(s, p, xq, ldq, xs, sms);
-    if (p.rows <= 128) return launch_skinny<128>(s, p, xq, ldq, xs, sms);
     const double big = tile_us(256, 2, p.rows, p.n, p.k, sms), mid = tile_us(128, 1, p.rows, p.n, p.k, sms),
                  low = tile_us(64, 1, p.rows, p.n, p.k, sms);
-    if (big <= mid && big <= low)
+    int nt = 0, split = 0;
+    if (p.rows <= 1024) {
+        const double few = skinny_us(p.rows, p.n, p.k, sms, nt, split);
+        if (few > big || few > mid || few > low) nt = 0;
+    }
+    if (nt == 16)
+        launch_skinny<16>(s, p, xq, ldq, xs, split);
+    else if (nt == 32)
+        launch_skinny<32>(s, p, xq, ldq, xs, split);
+    else if (nt == 64)
+        launch_skinny<64>(s, p, xq, ldq, xs, split);
+    else if (nt == 128)
+        launch_skinny<128>(s, p, xq, ldq, xs, split);
+    else if (big <= mid && big <= low)
         launch<256, 2>(s, p, xq, ldq, xs, sms);
     else if (mid <= low)
         launch<128, 1>(s, p, xq, ldq, xs, sms);

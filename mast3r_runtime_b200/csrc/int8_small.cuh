@@ -4,9 +4,9 @@
 // itself, into shared memory, while its first weights travel; a warp takes 4 output channels at a
 // time, its lanes 16 bytes of k each, and adds up four products an instruction.
 //
-// int8_skinny_kernel (up to 128 rows): the roles of the operands are exchanged -- 128 output
-// channels are the rows of the tensor-core tile, the tokens its NT columns -- so that a stage of
-// the pipeline is mostly weights.  A cluster of up to 8 CTAs splits k; each leaves its sums in
+// int8_skinny_kernel (few rows, or few tiles and a long k): the roles of the operands are exchanged --
+// 128 output channels are the rows of the tensor-core tile, up to NT tokens its columns -- so that with
+// few tokens a stage of the pipeline is mostly weights.  A cluster of up to 8 CTAs splits k; each leaves its sums in
 // shared memory, and every CTA adds and finishes some of the tokens from all of them (integer
 // sums: the order does not matter).
 #pragma once
@@ -25,7 +25,7 @@ __device__ __forceinline__ float finish1(int acc, float xs, float ws, float bias
     const float v = fmaf(static_cast<float>(acc) * xs, ws, bias);
     if (act == ACT_GELU) {
         const float u = v * fmaf(v * v, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-        if (f32) return v * __frcp_rn(1.0f + ex2_approx(-2.885390081777927f * u));
+        if (f32) return v * rcp_approx(1.0f + ex2_approx(-2.885390081777927f * u));
         float t;
         asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
         return fmaf(0.5f * v, t, 0.5f * v);
@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
 
 // ------------------------------------------------------------------------- skinny
 struct SkinnyParams {
-    int M, N, num_kb, split;  // k-blocks of 128 bytes, shared by `split` CTAs of a cluster
+    int M, N, tiles_n;
+    int num_kb, split;  // k-blocks of 128 bytes, shared by `split` CTAs of a cluster
     const float* xs;
     const float* ws;
     const float* bias;
@@ -281,7 +282,10 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     const int tid = threadIdx.x, warp = tid >> 5;
     const int split = p.split;
     const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
-    const int n0 = (blockIdx.x / split) * 128;
+    const int tile = blockIdx.x / split;
+    const int m0 = tile / p.tiles_n * NT;  // the tile's tokens and channels
+    const int n0 = tile % p.tiles_n * 128;
+    const int tokens = min(NT, p.M - m0);
     const int kb0 = static_cast<int>(static_cast<long long>(p.num_kb) * rank / split);
     const int kb1 = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / split);
 
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             tma_load_2d(sW + s * C::W_BYTES, &mapW, &full[s], (kb0 + s) * 128, n0);
         }
         grid_dependency_wait();
-        for (int s = 0; s < early; ++s) tma_load_2d(sX + s * C::X_BYTES, &mapX, &full[s], (kb0 + s) * 128, 0);
+        for (int s = 0; s < early; ++s) tma_load_2d(sX + s * C::X_BYTES, &mapX, &full[s], (kb0 + s) * 128, m0);
         bool ok = true;
         int it = early;
         for (int kb = kb0 + early; kb < kb1; ++kb, ++it) {
@@ -324,7 +328,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             }
             mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
             tma_load_2d(sW + s * C::W_BYTES, &mapW, &full[s], kb * 128, n0);
-            tma_load_2d(sX + s * C::X_BYTES, &mapX, &full[s], kb * 128, 0);
+            tma_load_2d(sX + s * C::X_BYTES, &mapX, &full[s], kb * 128, m0);
         }
         if (!ok) {  // drain: wait (bounded) for loads that may still be in flight
             volatile int dummy = 0;
@@ -386,27 +390,27 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     for (int r = 0; r < 8; ++r)
         peer[r] = cluster_addr(smem_u32(part + 4 * lane), static_cast<uint32_t>(r < split ? r : 0));
     constexpr int U = 2;  // tokens of a warp at once
-    for (int t0 = rank + split * warp; t0 < p.M; t0 += 4 * U * split) {
+    for (int t0 = rank + split * warp; t0 < tokens; t0 += 4 * U * split) {
         int4 v[U][8];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 const int t = t0 + u * 4 * split;
-                v[u][r] = r < split && t < p.M ? ld_cluster_int4(peer[r] + t * 512) : make_int4(0, 0, 0, 0);
+                v[u][r] = r < split && t < tokens ? ld_cluster_int4(peer[r] + t * 512) : make_int4(0, 0, 0, 0);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int t = t0 + u * 4 * split;
-            if (t >= p.M) continue;
+            if (t >= tokens) continue;
             int sum[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int r = 0; r < 8; ++r) sum[0] += v[u][r].x, sum[1] += v[u][r].y, sum[2] += v[u][r].z, sum[3] += v[u][r].w;
-            const float xs = p.xs[t];
+            const float xs = p.xs[m0 + t];
             float y[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) y[c] = finish1(sum[c], xs, ws[c], bias[c], p.act, p.out_dt == OP_F32);
-            const long long at = t * p.ldo + n0 + 4 * lane;
+            const long long at = (m0 + t) * p.ldo + n0 + 4 * lane;
             if (p.out_vec && n0 + 4 * lane + 4 <= p.N) {
                 if (p.out_dt == OP_F32)
                     *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(y[0], y[1], y[2], y[3]);

@@ -159,7 +159,8 @@ def linear64(q, s, w, ws, bias, act, out_dtype):
 SHAPES = [(1, 1, 1), (1, 5, 16), (1, 4096, 1024), (2, 130, 257), (3, 1153, 1000), (7, 64, 4096), (8, 1000, 33),
           (9, 300, 512), (16, 4096, 640), (17, 129, 2048), (24, 2048, 4096), (33, 520, 128), (64, 1000, 999),
           (65, 96, 384), (128, 1152, 384), (129, 257, 129), (577, 1153, 1000), (1536, 2304, 768), (2500, 4100, 1040),
-          (20000, 1040, 768), (19500, 1501, 1000), (26001, 600, 70)]
+          (20000, 1040, 768), (19500, 1501, 1000), (26001, 600, 70), (220, 360, 11869), (452, 961, 2880), (1000, 130, 16384),
+          (43, 316, 80), (129, 128, 4096)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
