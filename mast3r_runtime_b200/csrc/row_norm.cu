@@ -72,8 +72,8 @@ struct RowSlice {
             for (int i = 0; i < 8 * NCH; ++i) v[i] = has(i) ? to_f(p[i * GT]) : 0.0f;
         }
     }
-    // Values 8 c .. 8 c + 8 of a float vector as long as the row (zero behind its end), or `none`
-    // where there is no vector.
+    // Values 8 c .. 8 c + 8 of a float vector as long as the row (any of its values behind its end), or
+    // `none` where there is no vector.
     __device__ __forceinline__ void vector8(const float* p, int c, float none, float (&o)[8]) const {
         if (p == nullptr) {
 #pragma unroll
@@ -81,14 +81,62 @@ struct RowSlice {
         } else if constexpr (VEC) {
             const float4* q = reinterpret_cast<const float4*>(p + min(chunk(c), D - 8));
             const float4 a = __ldg(q), b = __ldg(q + 1);
-            const bool in = chunk(c) < D;
-            o[0] = in ? a.x : 0.0f, o[1] = in ? a.y : 0.0f, o[2] = in ? a.z : 0.0f, o[3] = in ? a.w : 0.0f;
-            o[4] = in ? b.x : 0.0f, o[5] = in ? b.y : 0.0f, o[6] = in ? b.z : 0.0f, o[7] = in ? b.w : 0.0f;
+            o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w;
+            o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
         } else {
             p += tid;
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j] = has(8 * c + j) ? __ldg(p + (8 * c + j) * GT) : 0.0f;
         }
+    }
+    // v summed over the thread's part of the row: values behind the row's end may be anything
+    __device__ __forceinline__ float part_sum(const float (&v)[8 * NCH]) const {
+        float t = 0.0f;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                float u = v[8 * c];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) u += v[8 * c + j];
+                t += chunk(c) < D ? u : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8 * NCH; ++i) t += has(i) ? v[i] : 0.0f;
+        }
+        return t;
+    }
+    __device__ __forceinline__ float part_square_sum(const float (&v)[8 * NCH]) const {
+        float t = 0.0f;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                float u = v[8 * c] * v[8 * c];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) u += v[8 * c + j] * v[8 * c + j];
+                t += chunk(c) < D ? u : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8 * NCH; ++i) t += has(i) ? v[i] * v[i] : 0.0f;
+        }
+        return t;
+    }
+    __device__ __forceinline__ float part_max(const float (&v)[8 * NCH]) const {
+        float t = 0.0f;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                float u = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u = max_abs(u, v[8 * c + j]);
+                t = max_abs(t, chunk(c) < D ? u : 0.0f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8 * NCH; ++i) t = max_abs(t, has(i) ? v[i] : 0.0f);
+        }
+        return t;
     }
     __device__ __forceinline__ void load_dt(int dt, const void* base, long long off, float (&v)[8 * NCH]) const {
         if (dt == OP_F32)
@@ -189,20 +237,12 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowRe
                                           int kind, float eps, const float* w, const float* b) {
     constexpr int N = 8 * NCH;
     const float inv_d = 1.0f / static_cast<float>(s.D);
-    float mean = 0.0f;
     if (kind == NORM_LAYER) {
-        float t = 0.0f;
+        const float mean = red.sum(s.part_sum(v)) * inv_d;
 #pragma unroll
-        for (int i = 0; i < N; ++i) t += v[i];
-        mean = red.sum(t) * inv_d;
+        for (int i = 0; i < N; ++i) v[i] -= mean;
     }
-    float q = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        v[i] = s.has(i) ? v[i] - mean : 0.0f;
-        q += v[i] * v[i];
-    }
-    const float rstd = rsqrtf(red.sum(q) * inv_d + eps);
+    const float rstd = rsqrtf(red.sum(s.part_square_sum(v)) * inv_d + eps);
     // the weight and bias vectors are read chunk by chunk: every row reads them from L1
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -217,11 +257,7 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowRe
 template <bool EXACT16, bool VEC, int NCH, int LANES, int GT>
 __device__ __forceinline__ void store_int8(const RowSlice<VEC, NCH, GT>& s, RowReduce<LANES>& red, const float (&v)[8 * NCH],
                                            int8_t* q, float* scale) {
-    constexpr int N = 8 * NCH;
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) m = max_abs(m, s.has(i) ? v[i] : 0.0f);
-    const uint32_t top = red.max(__float_as_uint(m) & 0x7FFFFFFFu);
+    const uint32_t top = red.max(__float_as_uint(s.part_max(v)) & 0x7FFFFFFFu);
     const bool live = live_magnitude(top);
     const Quantizer z(__uint_as_float(top));
     if (s.tid == 0) *scale = z.a / 127.0f;
@@ -292,7 +328,7 @@ __device__ __forceinline__ void row_body(const RowNormParams& p, const RowSlice<
 
 // LANES threads of a warp to a row (a few rows to a warp when it is short), or 0: a block.
 template <bool VEC, int NCH, int LANES, int MODE, int GT>
-__global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH == 4 && MODE == ROW_FULL ? 5 : 0)
+__global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH >= 3 && MODE == ROW_FULL ? 9 - NCH : 0)
     row_norm_kernel(const __grid_constant__ RowNormParams p) {
     if constexpr (MODE != ROW_FULL) {
         grid_dependency_wait();
@@ -417,6 +453,7 @@ void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
     if (p.cols <= 128) return launch<true, 1, 16>(s, p, 128);
     if (p.cols <= 256) return launch<true, 1, 32>(s, p, 128);
     if (p.cols <= 512 && p.rows > 148 * 16) return launch<true, 2, 32>(s, p, 128);
+    if (p.cols <= 768 && p.rows > 148 * (is_quantize(p) ? 16 : 32)) return launch<true, 3, 32>(s, p, 128);
     if (p.cols <= 1024 && p.rows > 148 * (is_quantize(p) ? 16 : 96)) return launch<true, 4, 32>(s, p, 128);
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
     if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, 0>(s, p, threads(1));
