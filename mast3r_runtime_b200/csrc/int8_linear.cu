@@ -85,28 +85,6 @@ __device__ __forceinline__ void tile_at(const Int8Params& p, int t, int& m, int&
     m = group * G + (r - n * gm);
 }
 
-// Pairs of 32-bit values in one instruction.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t p) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 constexpr float kGelu0 = 0.7978845608028654f;             // sqrt(2 / pi)
 constexpr float kGelu1 = 0.7978845608028654f * 0.044715f;
 

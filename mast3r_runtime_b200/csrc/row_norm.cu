@@ -95,10 +95,11 @@ struct RowSlice {
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                float u = v[8 * c];
+                uint64_t u = pair(v[8 * c], v[8 * c + 1]);
 #pragma unroll
-                for (int j = 1; j < 8; ++j) u += v[8 * c + j];
-                t += chunk(c) < D ? u : 0.0f;
+                for (int j = 2; j < 8; j += 2) u = add2(u, pair(v[8 * c + j], v[8 * c + j + 1]));
+                const float2 f = unpair(u);
+                t += chunk(c) < D ? f.x + f.y : 0.0f;
             }
         } else {
 #pragma unroll
@@ -111,10 +112,15 @@ struct RowSlice {
         if constexpr (VEC) {
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                float u = v[8 * c] * v[8 * c];
+                uint64_t u = pair(v[8 * c], v[8 * c + 1]);
+                u = mul2(u, u);
 #pragma unroll
-                for (int j = 1; j < 8; ++j) u += v[8 * c + j] * v[8 * c + j];
-                t += chunk(c) < D ? u : 0.0f;
+                for (int j = 2; j < 8; j += 2) {
+                    const uint64_t w = pair(v[8 * c + j], v[8 * c + j + 1]);
+                    u = fma2(w, w, u);
+                }
+                const float2 f = unpair(u);
+                t += chunk(c) < D ? f.x + f.y : 0.0f;
             }
         } else {
 #pragma unroll
@@ -232,6 +238,12 @@ struct RowReduce {
     }
 };
 
+template <int N>
+__device__ __forceinline__ void set(float (&v)[N], int i, uint64_t two) {
+    const float2 f = unpair(two);
+    v[i] = f.x, v[i + 1] = f.y;
+}
+
 template <bool VEC, int NCH, int LANES, int GT>
 __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowReduce<LANES>& red, float (&v)[8 * NCH],
                                           int kind, float eps, const float* w, const float* b) {
@@ -240,7 +252,7 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowRe
     if (kind == NORM_LAYER) {
         const float mean = red.sum(s.part_sum(v)) * inv_d;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] -= mean;
+        for (int i = 0; i < N; i += 2) set(v, i, add2(pair(v[i], v[i + 1]), pair(-mean, -mean)));
     }
     const float rstd = rsqrtf(red.sum(s.part_square_sum(v)) * inv_d + eps);
     // the weight and bias vectors are read chunk by chunk: every row reads them from L1
@@ -250,7 +262,10 @@ __device__ __forceinline__ void normalise(const RowSlice<VEC, NCH, GT>& s, RowRe
         s.vector8(w, c, 1.0f, g);
         s.vector8(b, c, 0.0f, a);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[8 * c + j] = v[8 * c + j] * rstd * g[j] + a[j];
+        for (int j = 0; j < 8; j += 2) {
+            const int i = 8 * c + j;
+            set(v, i, fma2(mul2(pair(v[i], v[i + 1]), pair(rstd, rstd)), pair(g[j], g[j + 1]), pair(a[j], a[j + 1])));
+        }
     }
 }
 
@@ -304,11 +319,16 @@ __device__ __forceinline__ void row_body(const RowNormParams& p, const RowSlice<
                     float gv[8];
                     s.vector8(g, c, 1.0f, gv);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[8 * c + j] = p.alpha * v[8 * c + j] + gv[j] * t[8 * c + j];
+                    for (int j = 0; j < 8; j += 2) {
+                        const int i = 8 * c + j;
+                        set(v, i, fma2(pair(gv[j], gv[j + 1]), pair(t[i], t[i + 1]),
+                                       mul2(pair(v[i], v[i + 1]), pair(p.alpha, p.alpha))));
+                    }
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = p.alpha * v[i] + t[i];
+                for (int i = 0; i < N; i += 2)
+                    set(v, i, fma2(pair(v[i], v[i + 1]), pair(p.alpha, p.alpha), pair(t[i], t[i + 1])));
             }
         } else {
 #pragma unroll
