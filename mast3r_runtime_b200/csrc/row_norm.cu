@@ -80,7 +80,7 @@ struct RowSlice {
             for (int j = 0; j < 8; ++j) o[j] = none;
         } else if constexpr (VEC) {
             const float4* q = reinterpret_cast<const float4*>(p + min(chunk(c), D - 8));
-            const float4 a = __ldg(q), b = __ldg(q + 1);
+            const float4 a = q[0], b = q[1];
             o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w;
             o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
         } else {
@@ -350,10 +350,8 @@ __device__ __forceinline__ void row_body(const RowNormParams& p, const RowSlice<
 template <bool VEC, int NCH, int LANES, int MODE, int GT>
 __global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH >= 3 && MODE == ROW_FULL ? 9 - NCH : 0)
     row_norm_kernel(const __grid_constant__ RowNormParams p) {
-    if constexpr (MODE != ROW_FULL) {
-        grid_dependency_wait();
-        grid_dependency_start();  // the product that follows may set itself up
-    }
+    if constexpr (VEC || MODE != ROW_FULL) grid_dependency_wait();
+    if constexpr (MODE != ROW_FULL) grid_dependency_start();  // the product that follows may set itself up
     __shared__ float red_buf[64];
     RowReduce<LANES> red(red_buf);
     const int tid = LANES ? static_cast<int>(threadIdx.x % (LANES ? LANES : 1)) : static_cast<int>(threadIdx.x);
@@ -368,7 +366,7 @@ __global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH >=
 
 // Many long rows: a block keeps its next rows of x and y on their way into shared memory with bulk
 // copies, so that the loads do not wait for the reductions of the row before and take no registers
-// (24,576 rows of 4,096, bf16: 132 us against 192; quantising alone gains nothing, 71 against 65).
+// (24,576 rows of 4,096, bf16: 129 us against 191; quantising alone gains nothing, 71 against 65).
 constexpr int kStreamStages = 4;
 
 __global__ void __launch_bounds__(1024) row_stream_kernel(const __grid_constant__ RowNormParams p, int stages) {
@@ -426,22 +424,26 @@ void launch(cudaStream_t s, const RowNormParams& p, int threads) {
     const long long per = LANES ? threads / (LANES ? LANES : 1) : 1;
     long long grid = (p.rows + per - 1) / per;
     if (grid > 148 * 64) grid = 148 * 64;
+    const LaunchConfig c(static_cast<unsigned>(grid), threads, 0, s);
     if (!is_quantize(p)) {
-        // an ordinary launch: it reads the weight vectors as constants (__ldg), which may come from the
-        // kernel before (without that, 199 us become 209 on 98,304 rows of 1,024)
-        row_norm_kernel<VEC, NCH, LANES, ROW_FULL, GT><<<static_cast<unsigned>(grid), threads, 0, s>>>(p);
-        M3R_CUDA(cudaGetLastError());
+        if constexpr (VEC) {
+            M3R_CUDA(cudaLaunchKernelEx(&c.cfg, row_norm_kernel<VEC, NCH, LANES, ROW_FULL, GT>, p));
+        } else {
+            // an ordinary launch: it reads the weight vectors as constants (__ldg), which may come from the
+            // kernel before (40,001 rows of 129: 21 us against 27 with plain loads)
+            row_norm_kernel<VEC, NCH, LANES, ROW_FULL, GT><<<static_cast<unsigned>(grid), threads, 0, s>>>(p);
+            M3R_CUDA(cudaGetLastError());
+        }
         return;
     }
     auto kern = p.x_dt == OP_F32 ? row_norm_kernel<VEC, NCH, LANES, ROW_QUANTIZE_F32, GT>
                                  : row_norm_kernel<VEC, NCH, LANES, ROW_QUANTIZE_16, GT>;
-    const LaunchConfig c(static_cast<unsigned>(grid), threads, 0, s);
     M3R_CUDA(cudaLaunchKernelEx(&c.cfg, kern, p));
 }
 
 // All of an SM's registers (64 a thread) in as many blocks as that makes, and shared memory but for
 // some that is left to L1, where the weight and gate vectors of every row come from (24,576 rows of
-// 4,096, bf16, with 225, 180 and 140 KB of rings: 140, 132, 133 us; 50,000 of 2,048: 145, 138, 148).
+// 4,096, bf16, with 225, 180 and 140 KB of rings: 133, 129, 128 us; 50,000 of 2,048: 134, 145, 142).
 // False where a block's share does not hold a row.
 bool launch_stream(cudaStream_t s, const RowNormParams& p, int threads) {
     constexpr int kMost = 180 * 1024;
@@ -462,23 +464,26 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
 }
 
 // Rows to threads.  Short rows share a warp, 8 values a lane.  With many rows, a warp each up to
-// 1,024 values (98,304 rows of 1,024, 32-bit stream: 199 us, against 226 with a block each); with
-// few, a block each, 8 values a thread, so that a row's chain of loads and reductions is short
-// (1,536 rows of 1,024 quantised: 4.0 us against 6.8; 6,144 rows of 1,024, whole operator: 18.5
-// against 20.4, 24,576: 57.8 against 55.4; 6,144 rows of 512: 9.7 either way; 12,288 of 1,024
-// quantised: 11 against 7 with a warp each).
+// 1,024 values (98,304 rows of 1,024, 32-bit stream: 188 us, against 209 with a block each; of 768: 141
+// against 158); with few, a block each, 8 values a thread, so that a row's chain of loads and reductions
+// is short (6,144 rows of 1,024: 17.7 us against 19.9, 12,288: 30.2 against 33.4, 24,576: 55.4 against
+// 55.9; 6,144 of 768: 14.5 to 15.6 against 12.1 to 15.9, by the norms; 6,144 of 512: 9.2 against 9.4).
+// Quantised only: 300 rows of 1,024 1.7 us with a block each against 1.8, 1,000 2.6 against 1.9, 32-bit
+// 2.65 against 2.7; 2,300 of 768 3.3 against 2.9.
 void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
     if (p.cols <= 32) return launch<true, 1, 4>(s, p, 128);
     if (p.cols <= 64) return launch<true, 1, 8>(s, p, 128);
     if (p.cols <= 128) return launch<true, 1, 16>(s, p, 128);
     if (p.cols <= 256) return launch<true, 1, 32>(s, p, 128);
+    const bool quantize = is_quantize(p);
+    const int few = p.x_dt == OP_F32 ? 12 : 4;  // rows an SM
     if (p.cols <= 512 && p.rows > 148 * 16) return launch<true, 2, 32>(s, p, 128);
-    if (p.cols <= 768 && p.rows > 148 * (is_quantize(p) ? 16 : 32)) return launch<true, 3, 32>(s, p, 128);
-    if (p.cols <= 1024 && p.rows > 148 * (is_quantize(p) ? 16 : 96)) return launch<true, 4, 32>(s, p, 128);
+    if (p.cols <= 768 && p.rows > 148 * (quantize ? few : 32)) return launch<true, 3, 32>(s, p, 128);
+    if (p.cols <= 1024 && p.rows > 148 * (quantize ? few : 96)) return launch<true, 4, 32>(s, p, 128);
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
     if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, 0>(s, p, threads(1));
     const int blocks = 148 * (1024 / threads(2));  // at 64 registers
-    if (p.rows >= 2LL * blocks && !is_quantize(p) && launch_stream(s, p, threads(2))) return;
+    if (p.rows >= 2LL * blocks && !quantize && launch_stream(s, p, threads(2))) return;
     launch<true, 2, 0>(s, p, threads(2));
 }
 
