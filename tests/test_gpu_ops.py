@@ -54,7 +54,8 @@ def levels(x):
 
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 127), (5, 256), (3, 513), (130, 1000), (67, 1024), (9, 1025),
-                                       (300, 4096), (2, 8200), (3, 16384), (1, 16383)])
+                                       (300, 4096), (2, 8200), (3, 16384), (1, 16383), (700, 768), (2000, 1000),
+                                       (9, 641), (5, 2345), (3, 5003)])
 def test_quantize_rows(ops, dtype, rows, cols):
     x = rnd(rows, cols, seed=rows + cols, dtype=DT[dtype])
     q, s = ops.quantize_rows(x)
@@ -260,7 +261,8 @@ def check_residual(ops, x, y, w, b, norm, out, **kw):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (9, 8), (1003, 32), (70, 31), (41, 64), (77, 100), (35, 128), (3, 33), (4, 256), (7, 384), (130, 1000), (65, 1001), (64, 1024),
-                                       (5, 1032), (301, 4096), (2, 4096), (3, 8191), (2, 16384)])
+                                       (5, 1032), (301, 4096), (2, 4096), (3, 8191), (2, 16384), (7, 641), (9, 1155),
+                                       (4, 1501), (5, 2345), (6, 3333), (3, 5003), (2, 9001), (5000, 552), (800, 768)])
 @pytest.mark.parametrize("norm,post", [("layer", None), ("rms", "rms"), ("layer", "layer")])
 def test_residual_norm(ops, rows, cols, norm, post):
     seed = rows * 7 + cols
@@ -318,7 +320,7 @@ def test_residual_norm_types_and_gates(ops, stream, branch):
     assert torch.equal(wide, keep)  # nothing beside the rows was written
 
 
-@pytest.mark.parametrize("cols", [24, 64, 65, 120, 1000, 1001, 4096])
+@pytest.mark.parametrize("cols", [24, 64, 65, 120, 768, 769, 1000, 1001, 3333, 4096])
 def test_residual_norm_in_8_bits(ops, cols):
     x, y = rnd(33, cols, seed=1), rnd(33, cols, seed=2, dtype=torch.bfloat16)
     x[5] = 0
