@@ -214,7 +214,9 @@ int m3r_residual_norm(const m3r_residual_norm_args* args) {
         p.ldy = a.ldy;
         p.ldr = a.ldr;
         p.ldo = a.ldo;
-        p.rows_per_gate = a.rows_per_gate > 0 ? a.rows_per_gate : std::numeric_limits<int64_t>::max();
+        // the kernel divides in 32 bits; rows are fewer, so that a larger group is one group
+        constexpr int64_t kOneGroup = std::numeric_limits<uint32_t>::max();
+        p.rows_per_gate = a.rows_per_gate > 0 && a.rows_per_gate < kOneGroup ? a.rows_per_gate : kOneGroup;
         p.ld_gate = a.rows_per_gate > 0 ? a.ld_gate : 0;
         p.x = a.x;
         p.y = a.y;

@@ -275,6 +275,27 @@ def test_residual_norm(ops, rows, cols, norm, post):
                    residual_scale=0.75, **kw)
 
 
+@pytest.mark.parametrize("per,groups", [(1, 6), (3, 2), (6, 1), (7, 1), (2 ** 32 - 1, 1), (2 ** 32, 1), (2 ** 33 + 2, 1)])
+def test_rows_of_a_gate_through_the_c_abi(ops, per, groups):
+    """Groups longer than the rows, past 32 bits too, are one group."""
+    from test_ops_args import RESIDUAL
+
+    from mast3r_runtime_b200 import _lib
+
+    rows, cols = 6, 40
+    x, y, gate = rnd(rows, cols, seed=1), rnd(rows, cols, seed=2), rnd(groups, cols, seed=3)
+    r, h = torch.empty_like(x), torch.empty_like(x)
+    lib = _lib.load()
+    args = RESIDUAL.pack(0, 2, 2, 2, 1, 0, 1e-6, 1.0, rows, cols, cols, cols, cols, cols, per, cols, x.data_ptr(),
+                         y.data_ptr(), gate.data_ptr(), 0, 0, 0, 0, r.data_ptr(), h.data_ptr(), 0,
+                         torch.cuda.current_stream().cuda_stream)
+    assert lib.m3r_residual_norm(args) == 0, lib.m3r_global_error()
+    r2, h2 = ops.residual_norm(x, y, None, gate=gate)
+    assert torch.equal(r, r2) and torch.equal(h, h2)
+    rows_gate = gate.double().repeat_interleave(rows // groups, 0)
+    assert (r.double() - (x.double() + rows_gate * y.double())).abs().max() <= 2 * U * (1 + 25)
+
+
 @pytest.mark.parametrize("rows,cols,stream,branch", [(2400, 1536, "fp32", "bf16"), (1300, 4096, "bf16", "fp16"),
                                                      (300, 16384, "fp32", "fp32"), (640, 8192, "fp16", "fp16")])
 def test_residual_norm_many_long_rows(ops, rows, cols, stream, branch):
