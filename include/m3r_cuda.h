@@ -309,7 +309,7 @@ int m3r_quantize_rows(const m3r_quantize_args* args);
 
 /* y[i, n] = act( (sum_k q_ik w_nk) * scale_i * w_scale_n + bias_n ), the sum exact in 32-bit
  * integers.  x in 16 or 32 bits is quantised row by row first (m3r_quantize_rows; k <= 16384)
- * into the workspace; x in 8 bits (rows 16-byte aligned, k <= 131072) comes with x_scale.
+ * into the workspace; x in 8 bits (rows 16-byte aligned, k <= 131071) comes with x_scale.
  * The weights' rows are 16-byte aligned: w a multiple of 16, ldw a multiple of 16 (pad the
  * rows of a k that is no multiple of 16; the padding is not used). */
 typedef struct m3r_int8_linear_args {

@@ -3,7 +3,7 @@
 //   y[i, n] = act( (sum_k q[i, k] w[n, k]) * s[i] * t[n] + bias[n] )
 //
 // x arrives as 8-bit rows with scales, or in 16 / 32 bits and is quantised row by row first
-// (row_norm.cu).  Sums are exact in 32-bit integers (k <= 131,072 keeps 127^2 k below 2^31).
+// (row_norm.cu).  Sums are exact in 32-bit integers (k <= 131,071 keeps 128^2 k below 2^31).
 //
 // Persistent tcgen05 kernel (kind::i8, twice the 16-bit rate): 320 threads -- warps 0-7
 // epilogue, warp 8 TMA producer, warp 9 TMEM allocator and MMA issuer -- on tiles of

@@ -15,6 +15,7 @@ enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 inline int op_size(int dt) { return dt == OP_F32 ? 4 : dt == OP_I8 ? 1 : 2; }
 
 constexpr int kRowMaxCols = 16384;  // longest row the row kernels hold in registers
+constexpr int64_t kInt8MaxK = 131071;  // sums of two 8-bit values, -128 among them, stay below 2^31
 
 // One pass over rows of `cols` values:  r = alpha x + gate * post(y),  h = norm(r) w + b.
 struct RowNormParams {

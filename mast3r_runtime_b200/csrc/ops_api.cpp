@@ -104,7 +104,7 @@ int64_t m3r_int8_linear_workspace(int x_dtype, int64_t rows, int64_t n, int64_t 
     const int rc = guarded([&] {
         M3R_REQUIRE(is_float(x_dtype) || x_dtype == M3R_DTYPE_I8, "int8_linear_workspace: unknown type of x");
         M3R_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 256 && n >= 1 && n < (int64_t(1) << 31) - 256 && k >= 1 &&
-                        k <= 131072,
+                        k <= m3r::kInt8MaxK,
                     "int8_linear_workspace: sizes out of range");
         bytes = static_cast<int64_t>(
             m3r::int8_linear_workspace(x_dtype, rows, static_cast<int>(n), static_cast<int>(k)));
@@ -122,8 +122,8 @@ int m3r_int8_linear(const m3r_int8_linear_args* args) {
         M3R_REQUIRE(a.rows >= 0 && a.rows < (int64_t(1) << 31) - 256, "int8_linear: rows out of range");
         M3R_REQUIRE(a.n >= 1 && a.n < (int64_t(1) << 31) - 256, "int8_linear: n out of range");
         const bool int8_x = a.x_dtype == M3R_DTYPE_I8;
-        M3R_REQUIRE(a.k >= 1 && a.k <= (int8_x ? 131072 : m3r::kRowMaxCols),
-                    "int8_linear: k out of range (1 to 131072 for 8-bit rows, to 16384 for rows to quantise)");
+        M3R_REQUIRE(a.k >= 1 && a.k <= (int8_x ? m3r::kInt8MaxK : m3r::kRowMaxCols),
+                    "int8_linear: k out of range (1 to 131071 for 8-bit rows, to 16384 for rows to quantise)");
         check_ld("int8_linear: x", a.ldx, a.k);
         check_ld("int8_linear: w", a.ldw, a.k);
         check_ld("int8_linear: out", a.ldo, a.n);

@@ -58,7 +58,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
     x in 16 or 32 bits is quantised row by row as quantize_rows does (k at most 16,384); x in int8
     comes with x_scale [...] (float32) and rows on 16-byte boundaries, as quantize_rows and
-    residual_norm return them (k at most 131,072).  weight is int8 [n, k] with rows on 16-byte
+    residual_norm return them (k at most 131,071).  weight is int8 [n, k] with rows on 16-byte
     boundaries and weight_scale float32 [n], as quantize_weight returns them; bias float32 [n].
     The sum over k is exact; scales, bias and activation ("none", "gelu" in its tanh form, "relu")
     are applied in 32 bits and rounded once to out_dtype (default: x's type, bfloat16 for int8)."""

@@ -190,12 +190,16 @@ def test_int8_linear_quantises_its_rows(ops, m, x, out, act, bias):
     close(y, want, tol)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 40, 16384), (5, 130, 131072), (200, 130, 131072)])
-def test_int8_linear_largest_sums(ops, m, n, k):
+@pytest.mark.parametrize("m,n,k", [(1, 40, 16384), (5, 130, 131071), (200, 130, 131071), (200, 130, 131056)])
+@pytest.mark.parametrize("least", [False, True])
+def test_int8_linear_largest_sums(ops, m, n, k, least):
     q, w = ints(m, k, 0, extreme=True), ints(n, k, 0, extreme=True)  # sums of 127^2 k, up to 2.1e9
+    top = 128.0 if least else 127.0
+    if least:
+        q.fill_(-128), w.fill_(-128)
     one = torch.ones(max(m, n), device="cuda")
     y = ops.int8_linear(q, w, one[:n], x_scale=one[:m], out_dtype=torch.float32)
-    assert (y.double() - 127.0 ** 2 * k).abs().max() <= U * 127.0 ** 2 * k
+    assert (y.double() - top ** 2 * k).abs().max() <= U * top ** 2 * k
 
 
 def test_int8_linear_layouts(ops):

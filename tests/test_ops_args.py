@@ -75,7 +75,7 @@ def test_c_refusals():
                       (dict(xt=3, xs=256, ldx=72), "16-byte aligned"), (dict(xt=3, xs=256, x=8), "16-byte aligned"),
                       (dict(work=0), "workspace"), (dict(size=64), "workspace"), (dict(work=320), "workspace"),
                       (dict(ldo=31), "stride"), (dict(ws=0), "null"), (dict(o=0), "null"), (dict(o=257), "misaligned"),
-                      (dict(b=257), "misaligned"), (dict(xt=3, xs=256, k=131073, ldx=131088, ldw=131088), "k out")):
+                      (dict(b=257), "misaligned"), (dict(xt=3, xs=256, k=131072, ldx=131072, ldw=131072), "k out")):
         refused("m3r_int8_linear", linear(**bad), text)
 
     def norm(xt=2, yt=0, ot=0, kind=1, post=0, eps=1e-6, alpha=1.0, rows=4, cols=8, ldx=8, ldy=8, ldr=8, ldo=8, per=0,
@@ -110,7 +110,7 @@ def test_workspace_sizes():
     f = _lib.load().m3r_int8_linear_workspace
     assert f(3, 100, 64, 64) == 0 and f(0, 0, 64, 64) == 0
     assert f(1, 1000, 64, 1001) >= 1000 * 1008 + 4000
-    for bad in ((4, 1, 1, 1), (0, -1, 1, 1), (0, 1, 0, 1), (0, 1, 1, 0), (0, 1, 1, 131073)):
+    for bad in ((4, 1, 1, 1), (0, -1, 1, 1), (0, 1, 0, 1), (0, 1, 1, 0), (0, 1, 1, 131072)):
         assert f(*bad) == -1
 
 
