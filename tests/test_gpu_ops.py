@@ -264,7 +264,8 @@ def check_residual(ops, x, y, w, b, norm, out, **kw):
     return r, h
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (9, 8), (1003, 32), (70, 31), (41, 64), (77, 100), (35, 128), (3, 33), (4, 256), (7, 384), (130, 1000), (65, 1001), (64, 1024),
+@pytest.mark.parametrize("rows,cols", [(1, 1), (9, 8), (1003, 32), (70, 31), (41, 64), (77, 100), (35, 128), (3, 33),
+                                       (4, 256), (7, 384), (130, 1000), (65, 1001), (64, 1024),
                                        (5, 1032), (301, 4096), (2, 4096), (3, 8191), (2, 16384), (7, 641), (9, 1155),
                                        (4, 1501), (5, 2345), (6, 3333), (3, 5003), (2, 9001), (5000, 552), (800, 768)])
 @pytest.mark.parametrize("norm,post", [("layer", None), ("rms", "rms"), ("layer", "layer")])
@@ -529,6 +530,49 @@ def test_same_inputs_give_the_same_bits(ops):
     first = block_entry(ops, s)
     for _ in range(5):
         assert all(torch.equal(i, j) for i, j in zip(first, block_entry(ops, s)))
+
+
+def test_captured_behind_copies_fills_and_joined_streams(ops):
+    """The kernels ahead of an operator may be no kernels (a copy, a fill) or several (a join)."""
+    rows, k, n = 50, 512, 200
+    src, x, y = rnd(rows, k, seed=1), torch.empty(rows, k, device="cuda"), torch.empty(rows, k, device="cuda")
+    w, ws = ops.quantize_weight(rnd(n, k, seed=2))
+    g1 = 1 + 0.1 * rnd(k, seed=3)
+    pos = torch.arange(rows, device="cuda")
+    freq = ops.rope_frequencies(100)[0]
+    side = torch.cuda.Stream()
+
+    def run():
+        now = torch.cuda.current_stream()
+        x.copy_(src)
+        q0, _ = ops.quantize_rows(x)            # behind a copy
+        y.zero_()
+        r0, h0 = ops.residual_norm(x, y, g1)    # behind a fill
+        side.wait_stream(now)
+        with torch.cuda.stream(side):
+            y.copy_(src)
+            p0 = ops.int8_linear(h0, w, ws)
+        z = x * 2
+        now.wait_stream(side)
+        r1, h1 = ops.residual_norm(z, y, g1)    # behind two kernels
+        p1 = ops.int8_linear(h1, w, ws)
+        t, _ = ops.rope(p1.view(rows, 2, 100), None, pos, freq)
+        return q0, r0, h0, p0, r1, h1, p1, t
+
+    want = [v.clone() for v in run()]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for seed in (1, 7):
+        src.copy_(rnd(rows, k, seed=seed))
+        if seed != 1:
+            want = [v.clone() for v in run()]
+        x.fill_(9), y.fill_(9)
+        for _ in range(3):
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @pytest.mark.parametrize("rows", [1, 3, 24, 100, 600, 20000])
