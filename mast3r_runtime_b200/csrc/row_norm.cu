@@ -465,9 +465,12 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
 
 // Rows to threads.  Short rows share a warp, 8 values a lane.  With many rows, a warp each up to
 // 1,024 values (98,304 rows of 1,024, 32-bit stream: 188 us, against 209 with a block each; of 768: 141
-// against 158); with few, a block each, 8 values a thread, so that a row's chain of loads and reductions
-// is short (6,144 rows of 1,024: 17.7 us against 19.9, 12,288: 30.2 against 33.4, 24,576: 55.4 against
-// 55.9; 6,144 of 768: 14.5 to 15.6 against 12.1 to 15.9, by the norms; 6,144 of 512: 9.2 against 9.4).
+// against 158); with few, a block each, so that a row's chain of loads and reductions is short: 8 values a
+// thread while an SM holds all its rows at once (592 rows of 1,024, bf16 stream and two norms: 3.2 us, 3.8
+// with 16 values), 16 above, where twice the rows are under way (2,304 rows: 7.1 and 6.1; 6,144: 18.2 and
+// 17.5, 18.0 with a warp each; 32-bit stream, one norm: 6.9 and 6.6, 17.4, 17.8 and 19.3).  Of 768: 2,304
+// rows 6.1 with a block each, 4.8 with a warp, 4,608 9.9 and 9.2; 32-bit 5.8 and 5.1, 10.5 and 11.9.
+// More rows than that again are copied ahead (9,216 of 1,024, bf16: 23.7 and 22.7).
 // Quantised only: 300 rows of 1,024 1.7 us with a block each against 1.8, 1,000 2.6 against 1.9, 32-bit
 // 2.65 against 2.7; 2,300 of 768 3.3 against 2.9.
 void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
@@ -476,12 +479,13 @@ void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
     if (p.cols <= 128) return launch<true, 1, 16>(s, p, 128);
     if (p.cols <= 256) return launch<true, 1, 32>(s, p, 128);
     const bool quantize = is_quantize(p);
-    const int few = p.x_dt == OP_F32 ? 12 : 4;  // rows an SM
+    const int few = p.x_dt == OP_F32 ? (quantize ? 12 : 32) : quantize ? 4 : 12;  // rows an SM
     if (p.cols <= 512 && p.rows > 148 * 16) return launch<true, 2, 32>(s, p, 128);
-    if (p.cols <= 768 && p.rows > 148 * (quantize ? few : 32)) return launch<true, 3, 32>(s, p, 128);
+    if (p.cols <= 768 && p.rows > 148 * few) return launch<true, 3, 32>(s, p, 128);
     if (p.cols <= 1024 && p.rows > 148 * (quantize ? few : 96)) return launch<true, 4, 32>(s, p, 128);
     auto threads = [&](int nch) { return ((p.cols + 8 * nch - 1) / (8 * nch) + 31) / 32 * 32; };
-    if (p.cols <= 1024 || (p.cols <= 8192 && p.rows <= 148 * 2)) return launch<true, 1, 0>(s, p, threads(1));
+    if (p.cols <= 1024 ? p.rows <= 148 * 8 || p.cols <= 768 || quantize : p.cols <= 8192 && p.rows <= 148 * 2)
+        return launch<true, 1, 0>(s, p, threads(1));
     const int blocks = 148 * (1024 / threads(2));  // at 64 registers
     if (p.rows >= 2LL * blocks && !quantize && launch_stream(s, p, threads(2))) return;
     launch<true, 2, 0>(s, p, threads(2));

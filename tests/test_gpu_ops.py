@@ -302,7 +302,9 @@ def test_rows_of_a_gate_through_the_c_abi(ops, per, groups):
 
 
 @pytest.mark.parametrize("rows,cols,stream,branch", [(2400, 1536, "fp32", "bf16"), (1300, 4096, "bf16", "fp16"),
-                                                     (300, 16384, "fp32", "fp32"), (640, 8192, "fp16", "fp16")])
+                                                     (300, 16384, "fp32", "fp32"), (640, 8192, "fp16", "fp16"),
+                                                     (5000, 1024, "fp32", "bf16"), (4801, 776, "fp32", "fp32"),
+                                                     (1300, 1000, "bf16", "bf16")])
 def test_residual_norm_many_long_rows(ops, rows, cols, stream, branch):
     """More rows than blocks fit the device: each block works through several, some copied ahead."""
     x, y = rnd(rows, cols, seed=1, dtype=DT[stream]), rnd(rows, cols, seed=2, dtype=DT[branch])
