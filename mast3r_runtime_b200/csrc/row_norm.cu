@@ -494,7 +494,8 @@ void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
 // Element accesses (odd widths, rows off the 16-byte grid): 8 or 16 values a thread, neighbouring
 // threads at neighbouring elements.  Threads without a value cost as much as the others, so the blocks
 // come in steps of a quarter to a half (24,576 rows of 513: 56 us in 128 threads, 44 in 96;
-// 5,000 of 5,003: 115 us with 8 values in 704 threads, which an SM holds once, 79 with 16 in 320).
+// 5,000 of 5,003: 115 us with 8 values in 704 threads, which an SM holds once, 79 with 16 in 320; 9,000 of
+// 2,005, bf16 stream: 67 and 52; 4,039 of 1,001 with 16 values: 18.4 against 16.5).
 template <int NCH, int GT>
 void launch_elements(cudaStream_t s, const RowNormParams& p) {
     launch<false, NCH, 0, GT>(s, p, GT);
@@ -509,9 +510,9 @@ void dispatch_elements(cudaStream_t s, const RowNormParams& p) {
     if (p.cols <= 8 * 96) return launch_elements<1, 96>(s, p);
     if (p.cols <= 8 * 128) return launch_elements<1, 128>(s, p);
     if (p.cols <= 8 * 160) return launch_elements<1, 160>(s, p);
-    if (p.cols <= 8 * 192) return launch_elements<1, 192>(s, p);
-    if (p.cols <= 8 * 256) return launch_elements<1, 256>(s, p);
-    if (p.cols <= 8 * 320) return launch_elements<1, 320>(s, p);
+    if (p.cols <= 16 * 96) return launch_elements<2, 96>(s, p);
+    if (p.cols <= 16 * 128) return launch_elements<2, 128>(s, p);
+    if (p.cols <= 16 * 160) return launch_elements<2, 160>(s, p);
     if (p.cols <= 16 * 256) return launch_elements<2, 256>(s, p);
     if (p.cols <= 16 * 320) return launch_elements<2, 320>(s, p);
     if (p.cols <= 16 * 512) return launch_elements<2, 512>(s, p);
