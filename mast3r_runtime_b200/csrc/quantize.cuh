@@ -42,9 +42,9 @@ struct Quantizer {
     // The quotient t / top for t = k v: for 16-bit v, t, the remainder and a quotient halfway between
     // two levels are exact in 32 bits, and any other quotient is 2^-19 away from half a level, so that
     // one correction makes its nearest integer the right one.
-    __device__ __forceinline__ float quotient16(float v) const {
-        const float t = v * k, q = t * inv;
-        return fmaf(fmaf(-q, top, t), inv, q);
+    __device__ __forceinline__ uint64_t quotient16(uint64_t v) const {  // two values
+        const uint64_t t = mul2(v, pair(k, k)), i = pair(inv, inv), q = mul2(t, i);
+        return fma2(fma2(q, pair(-top, -top), t), i, q);
     }
 };
 
@@ -58,14 +58,19 @@ __device__ __forceinline__ uint2 quantize8(const float* v, const Quantizer& z) {
     uint32_t b[8];
     if constexpr (EXACT16) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(z.quotient16(v[j]) + kMagic);
+        for (int j = 0; j < 8; j += 2) {
+            const float2 t = unpair(add2(z.quotient16(pair(v[j], v[j + 1])), pair(kMagic, kMagic)));
+            b[j] = __float_as_uint(t.x), b[j + 1] = __float_as_uint(t.y);
+        }
     } else {
         float off = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float p = v[j] * z.k * z.inv, t = p + kMagic;
-            off = fmaxf(off, fabsf(p - (t - kMagic)));
-            b[j] = __float_as_uint(t);
+        for (int j = 0; j < 8; j += 2) {
+            const uint64_t p = mul2(mul2(pair(v[j], v[j + 1]), pair(z.k, z.k)), pair(z.inv, z.inv));
+            const uint64_t t = add2(p, pair(kMagic, kMagic));
+            const float2 d = unpair(fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f), p)), u = unpair(t);
+            off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+            b[j] = __float_as_uint(u.x), b[j + 1] = __float_as_uint(u.y);
         }
         if (off > 0.49996f) {
 #pragma unroll

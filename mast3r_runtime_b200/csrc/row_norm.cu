@@ -346,9 +346,15 @@ __device__ __forceinline__ void row_body(const RowNormParams& p, const RowSlice<
     }
 }
 
+// At least this many blocks an SM: a warp's row in 64 to 96 registers; a block's 16-bit row to quantise in 32,
+// so that all of an SM's threads load (24,576 rows of 4,096: 59 us, 72 with 43 registers).
+constexpr int row_blocks(bool vec, int nch, int lanes, int mode) {
+    return lanes && nch >= 3 && mode == ROW_FULL ? 9 - nch : vec && lanes == 0 && mode == ROW_QUANTIZE_16 ? 2 : 0;
+}
+
 // LANES threads of a warp to a row (a few rows to a warp when it is short), or 0: a block.
 template <bool VEC, int NCH, int LANES, int MODE, int GT>
-__global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH >= 3 && MODE == ROW_FULL ? 9 - NCH : 0)
+__global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, row_blocks(VEC, NCH, LANES, MODE))
     row_norm_kernel(const __grid_constant__ RowNormParams p) {
     if constexpr (VEC || MODE != ROW_FULL) grid_dependency_wait();
     if constexpr (MODE != ROW_FULL) grid_dependency_start();  // the product that follows may set itself up
@@ -366,7 +372,7 @@ __global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, LANES && NCH >=
 
 // Many long rows: a block keeps its next rows of x and y on their way into shared memory with bulk
 // copies, so that the loads do not wait for the reductions of the row before and take no registers
-// (24,576 rows of 4,096, bf16: 129 us against 191; quantising alone gains nothing, 71 against 65).
+// (24,576 rows of 4,096, bf16: 129 us against 191; quantising alone gains nothing, 71 against 59).
 constexpr int kStreamStages = 4;
 
 __global__ void __launch_bounds__(1024) row_stream_kernel(const __grid_constant__ RowNormParams p, int stages) {
