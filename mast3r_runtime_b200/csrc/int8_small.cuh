@@ -21,14 +21,12 @@ namespace m3r {
 namespace {
 
 // y = act(acc * xs * ws + bias), one value
-__device__ __forceinline__ float finish1(int acc, float xs, float ws, float bias, int act, bool f32) {
+__device__ __forceinline__ float finish1(int acc, float xs, float ws, float bias, int act) {
     const float v = fmaf(static_cast<float>(acc) * xs, ws, bias);
     if (act == ACT_GELU) {
+        // x / 2 (1 + tanh u) as x / (1 + exp(-2 u)), which loses no digits where the tanh nears -1
         const float u = v * fmaf(v * v, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-        if (f32) return v * rcp_approx(1.0f + ex2_approx(-2.885390081777927f * u));
-        float t;
-        asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
-        return fmaf(0.5f * v, t, 0.5f * v);
+        return v * rcp_approx(1.0f + ex2_approx(-2.885390081777927f * u));
     }
     if (act == ACT_RELU) return v < 0.0f ? 0.0f : v;  // keeps NaN
     return v;
@@ -219,8 +217,7 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
         const int n = first + lane / MR, m = lane % MR;
         if (lane < kGemvCols * MR && n < p.N && m < p.M) {
             const float b = p.bias ? p.bias[n] : 0.0f;
-            store1(p.out, p.out_dt, m * p.ldo + n,
-                   finish1(mine, scale[m], p.ws[n], b, p.act, p.out_dt == OP_F32));
+            store1(p.out, p.out_dt, m * p.ldo + n, finish1(mine, scale[m], p.ws[n], b, p.act));
         }
     }
 }
@@ -409,7 +406,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             const float xs = p.xs[m0 + t];
             float y[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) y[c] = finish1(sum[c], xs, ws[c], bias[c], p.act, p.out_dt == OP_F32);
+            for (int c = 0; c < 4; ++c) y[c] = finish1(sum[c], xs, ws[c], bias[c], p.act);
             const long long at = (m0 + t) * p.ldo + n0 + 4 * lane;
             if (p.out_vec && n0 + 4 * lane + 4 <= p.N) {
                 if (p.out_dt == OP_F32)

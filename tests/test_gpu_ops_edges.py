@@ -1,0 +1,71 @@
+"""GPU tests of the operators at the edges of their ranges: results far below the values they are
+made from, columns that are not finite.
+
+Tolerances count roundings as test_gpu_ops.py does: U = 2^-24 is one 32-bit rounding, half(dtype)
+half a step of the result's type."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_ops import DT, U, close, half, ops  # noqa: E402,F401
+
+
+# ----------------------------------------------------------------------------- GELU
+def gelu64(v):
+    """v * sigmoid(2 u), u = sqrt(2 / pi) (v + 0.044715 v^3), which loses nothing where 1 + tanh(u)
+    does, and the bound of its 32-bit form: the argument 2 u has 8 roundings (constants among them),
+    the exponential 2^-22, reciprocal and products 16 U; v itself one, which the value's slope
+    enlarges."""
+    u2 = 2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+    y = v * torch.sigmoid(u2)
+    slope = 1 + v.abs() * 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * v * v)
+    return y, y.abs() * (8 * U * u2.abs() + 16 * U + 2 * U * slope)
+
+
+def gelu_inputs(m, n):
+    """8-bit rows and weights whose sums are one product each: column j of row i holds q_i * 127 * ws_j,
+    from -12 to 12."""
+    q = torch.zeros(m, 16, dtype=torch.int8)
+    q[:, 0] = (torch.arange(m) * 37 % 255 - 127).to(torch.int8) if m > 4 else torch.tensor([-127, -64, -31, 90])[:m]
+    w = torch.zeros(n, 16, dtype=torch.int8)
+    w[:, 0] = 127
+    ws = (torch.arange(n) + 1) * (12 / 127 / 127 / n)
+    return q.cuda(), w.cuda(), ws.float().cuda()
+
+
+# the one-launch kernel, the one that splits k, tiles of one CTA and of a pair
+GELU_SHAPES = [(1, 40), (4, 200), (24, 200), (255, 300), (3000, 130), (20000, 1024)]
+
+
+@pytest.mark.parametrize("m,n", GELU_SHAPES)
+@pytest.mark.parametrize("out", DT)
+def test_gelu_of_negative_values_keeps_its_digits(ops, m, n, out):  # noqa: F811
+    """Each result is right to its own size, down to the ones far below the values they come from."""
+    q, w, ws = gelu_inputs(m, n)
+    y = ops.int8_linear(q, w, ws, x_scale=torch.ones(m, device="cuda"), act="gelu", out_dtype=DT[out])
+    v = q[:, :1].double() * 127 * ws.double()
+    want, tol = gelu64(v)
+    # half a step of fp16's smallest values; results below 2^-120 may be zero
+    least = 2.0 ** -25 if out == "fp16" else 2.0 ** -120
+    close(y, want, tol + half(DT[out]) * (want.abs() + tol) + least)
+
+
+@pytest.mark.parametrize("m,n", GELU_SHAPES)
+@pytest.mark.parametrize("out", DT)
+def test_gelu_columns_that_are_not_finite_stay_alone(ops, m, n, out):  # noqa: F811
+    q, w, ws = gelu_inputs(m, n)
+    one = torch.ones(m, device="cuda")
+    y = ops.int8_linear(q, w, ws, x_scale=one, act="gelu", out_dtype=DT[out])
+    ws[5], ws[18] = math.nan, math.inf
+    z = ops.int8_linear(q, w, ws, x_scale=one, act="gelu", out_dtype=DT[out])
+    keep = [j for j in range(n) if j not in (5, 18)]
+    assert torch.equal(z[:, keep], y[:, keep])
+    assert torch.isnan(z[:, 5]).all()
+    up = q[:, 0] > 0
+    assert torch.isposinf(z[up, 18]).all() and torch.isnan(z[~up, 18]).all()
