@@ -11,6 +11,7 @@
 // sums: the order does not matter).
 #pragma once
 
+#include "column_walk.h"
 #include "common.cuh"
 #include "gemm.cuh"
 #include "ops.h"
@@ -126,13 +127,14 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
     __shared__ float scale[MR];
     __shared__ uint32_t part[kGemvThreads / 32][MR];
     const int tid = threadIdx.x, lane = tid & 31;
-    const int warps = gridDim.x * (kGemvThreads / 32);
     const int chunks = p.K / 16, tail = p.K % 16;  // whole 16 bytes of k, and what is left
-    int n0 = (blockIdx.x * (kGemvThreads / 32) + (tid >> 5)) * kGemvCols;
+    const uint32_t warps = gridDim.x * (kGemvThreads / 32);
+    ColumnWalk cols{(blockIdx.x * (kGemvThreads / 32) + (tid >> 5)) * kGemvCols, warps * kGemvCols,
+                    static_cast<uint32_t>(p.N)};
 
     // two steps of 16 bytes a lane for each channel; channels past the end read the last one
     uint4 w[kGemvCols][2];
-    auto channel = [&](int i) { return p.w + static_cast<long long>(min(n0 + i, p.N - 1)) * p.ldw; };
+    auto channel = [&](int i) { return p.w + static_cast<long long>(cols.column(i)) * p.ldw; };
     auto load = [&](int c) {
 #pragma unroll
         for (int i = 0; i < kGemvCols; ++i) {
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
         }
     };
     grid_dependency_wait();
-    if (n0 < p.N) load(lane);
+    if (cols.live()) load(lane);
     if (p.x_dt == OP_I8) {
         for (int m = 0; m < MR; ++m) {
             const int8_t* row = static_cast<const int8_t*>(p.x) + m * p.ldx;
@@ -161,14 +163,14 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
     }
     __syncthreads();
 
-    while (n0 < p.N) {
+    while (cols.live()) {
         int acc[kGemvCols][MR] = {};
         const int8_t* last[kGemvCols];
         if (tail) {
 #pragma unroll
             for (int i = 0; i < kGemvCols; ++i) last[i] = channel(i) + chunks * 16;
         }
-        const int first = n0;
+        const uint32_t first = cols.at;
         for (int c = lane; c - lane < chunks; c += 64) {
             uint4 a[kGemvCols][2];
 #pragma unroll
@@ -177,8 +179,8 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
             if (c - lane + 64 < chunks) {
                 load(c + 64);
             } else {
-                n0 += warps * kGemvCols;
-                if (n0 < p.N) load(lane);
+                cols.next();
+                if (cols.live()) load(lane);
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
                 }
             }
         }
-        if (chunks == 0) n0 += warps * kGemvCols;
+        if (chunks == 0) cols.next();
         if (lane < tail) {
 #pragma unroll
             for (int i = 0; i < kGemvCols; ++i)
@@ -214,8 +216,9 @@ __global__ void __launch_bounds__(kGemvThreads) int8_gemv_kernel(const __grid_co
                 const int sum = __reduce_add_sync(0xffffffffu, acc[i][m]);
                 if (lane == i * MR + m) mine = sum;
             }
-        const int n = first + lane / MR, m = lane % MR;
-        if (lane < kGemvCols * MR && n < p.N && m < p.M) {
+        const uint32_t n = first + lane / MR;
+        const int m = lane % MR;
+        if (lane < kGemvCols * MR && n < cols.n && m < p.M) {
             const float b = p.bias ? p.bias[n] : 0.0f;
             store1(p.out, p.out_dt, m * p.ldo + n, finish1(mine, scale[m], p.ws[n], b, p.act));
         }

@@ -153,3 +153,43 @@ def test_rope_frequencies():
                 dict(rot_dim=8, factor=0.5), dict(rot_dim=8, base=0.0), dict(rot_dim=8, axes=3)):
         with pytest.raises(ValueError):
             ops.rope_frequencies(**bad, device="cpu")
+
+
+def test_column_walk_near_the_largest_n(tmp_path):
+    """The few-row product accepts n up to 2^31 - 257: no warp leaves the columns, and each column is
+    one warp's."""
+    src = tmp_path / "walk.cpp"
+    src.write_text(textwrap.dedent("""
+        #include <stdint.h>
+        #include <stdio.h>
+        #include <initializer_list>
+        #include "column_walk.h"
+        // the last column that the warp starting at `at` reaches, or -1 when a group lies outside
+        static long long last(uint32_t at, uint32_t step, uint32_t n) {
+          m3r::ColumnWalk w{at, step, n};
+          long long groups = 0, end = 0;
+          for (; w.live(); w.next()) {
+            for (uint32_t i = 0; i < 4; ++i)
+              if (w.column(i) >= n || (long long)w.column(i) < end) return -1;
+            end = w.column(3);
+            if (++groups > (long long)n / step + 1) return -1;
+          }
+          return groups == (n - at + step - 1LL) / step ? end : -1;
+        }
+        int main() {
+          const uint32_t step = 148 * 2 * 8 * 4;
+          const uint32_t ns[] = {2147483391u, 2147483391u - 9471u, 2147474176u, 2147483390u, 9473u, 5u};
+          for (uint32_t n : ns)
+            for (uint32_t at : {0u, 4u, step / 2, step - 8, step - 4})
+              if (at < n) {
+                const long long e = last(at, step, n);
+                if (e < 0 || e >= n || e + step < n) return printf("n %u from %u: %lld\\n", n, at, e), 1;
+              }
+          return 0;
+        }
+    """))
+    exe = tmp_path / "walk"
+    csrc = ROOT / "mast3r_runtime_b200" / "csrc"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(csrc), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stdout
