@@ -241,7 +241,7 @@ int m3r_rope(const m3r_rope_args* args) {
         M3R_REQUIRE(a.axes == 1 || a.axes == 2, "rope: axes must be 1 or 2");
         M3R_REQUIRE(a.pos_bits == 32 || a.pos_bits == 64, "rope: positions must be 32- or 64-bit integers");
         M3R_REQUIRE(a.dim >= 2 && a.dim <= 4096, "rope: head size out of range (2 to 4096)");
-        M3R_REQUIRE(a.n_freq >= 1 && 2 * a.n_freq <= a.dim, "rope: more frequencies than pairs of the head");
+        M3R_REQUIRE(a.n_freq >= 1 && a.n_freq <= a.dim / 2, "rope: more frequencies than pairs of the head");
         M3R_REQUIRE(a.axes == 1 || a.n_freq % 2 == 0, "rope: two axes need an even number of frequencies");
         M3R_REQUIRE(a.batch >= 0 && a.tokens >= 0 && a.batch < (int64_t(1) << 31) && a.tokens < (int64_t(1) << 31) &&
                         a.batch * a.tokens < (int64_t(1) << 31) - 64,

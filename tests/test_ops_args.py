@@ -193,3 +193,9 @@ def test_column_walk_near_the_largest_n(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(csrc), str(src), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert out.returncode == 0, out.stdout
+
+
+@pytest.mark.parametrize("n_freq", [2 ** 62, 2 ** 62 + 16, 2 ** 63 - 1, 2 ** 32 + 16, 33])
+def test_rope_frequency_counts_that_do_not_fit_32_bits(n_freq):
+    refused("m3r_rope", ROPE.pack(0, 0, 0, 1, 64, 1.0, 1, 4, 64, n_freq, 0, 0, 1, 16, 16, 16, 16, 2, 0, 128, 64, 0, 128,
+                                  64, *(0,) * 9, 0), "more frequencies")
