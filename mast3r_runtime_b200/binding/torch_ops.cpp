@@ -13,10 +13,12 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <initializer_list>
 #include <stdexcept>
 #include <string>
+#include <utility>
 
 #include "../../include/m3r_cuda.h"
 
@@ -60,12 +62,108 @@ int64_t device_of(const char* op, std::initializer_list<const Tensor*> all) {
     return dev;
 }
 
+// One term of a sum of whole multiples of steps (bytes): step * x with lo <= x <= hi.
+struct Term {
+    int64_t step, lo, hi;
+};
+
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }  // b > 0
+
+// Whether the terms can add up to `target`; `moved`: so that an x other than the last term's is not zero.
+// Terms come by falling step, so that with the steps of ordinary layouts (each beyond what the smaller
+// ones reach together) two or three values of an x are tried; sums that take more than `budget` trials
+// count as possible.
+bool adds_up(const Term* t, size_t n, int64_t target, bool moved, int& budget) {
+    if (n == 0) return target == 0 && moved;
+    if (--budget < 0) return true;
+    int64_t lo = 0, hi = 0;  // of the terms behind this one
+    for (size_t i = 1; i < n; ++i) {
+        lo += t[i].step * t[i].lo;
+        hi += t[i].step * t[i].hi;
+    }
+    const int64_t first = std::max(t->lo, -floor_div(hi - target, t->step));
+    const int64_t last = std::min(t->hi, floor_div(target - lo, t->step));
+    for (int64_t x = first; x <= last; ++x)
+        if (adds_up(t + 1, n - 1, target - t->step * x, moved || (x != 0 && n > 1), budget)) return true;
+    return false;
+}
+
+constexpr int kOverlapTrials = 20000;
+
+bool by_step(const Term& a, const Term& b) { return a.step > b.step; }
+
+// Whether two of a tensor's elements share memory.
+bool overlaps_itself(const Tensor& t) {
+    if (t.numel() <= 1 || t.is_non_overlapping_and_dense()) return false;
+    const int64_t size = static_cast<int64_t>(t.element_size());
+    c10::SmallVector<Term, 8> terms;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+        if (t.size(i) == 1) continue;
+        if (t.stride(i) == 0) return true;
+        terms.push_back({t.stride(i) * size, 1 - t.size(i), t.size(i) - 1});
+    }
+    std::sort(terms.begin(), terms.end(), by_step);
+    terms.push_back({1, 1 - size, size - 1});
+    int budget = kOverlapTrials;
+    return adds_up(terms.data(), terms.size(), 0, false, budget);
+}
+
+struct Extent {
+    int64_t begin, end;  // bytes
+    explicit Extent(const Tensor& t) : begin(reinterpret_cast<int64_t>(t.const_data_ptr())), end(begin) {
+        for (int64_t i = 0; i < t.dim(); ++i) end += (t.size(i) - 1) * t.stride(i) * static_cast<int64_t>(t.element_size());
+        end += static_cast<int64_t>(t.element_size());
+    }
+};
+
+// Whether an element of `a` shares memory with one of `b`.  Views of one projection lie between one
+// another without that.
+bool overlaps(const Tensor& a, const Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const Extent ea(a), eb(b);
+    if (ea.end <= eb.begin || eb.end <= ea.begin) return false;
+    c10::SmallVector<Term, 16> terms;
+    // a's address less b's: a step that both have is one term
+    auto add = [&](int64_t step, int64_t lo, int64_t hi) {
+        if (step == 0) return;
+        for (Term& t : terms)
+            if (t.step == step) {
+                t.lo += lo;
+                t.hi += hi;
+                return;
+            }
+        terms.push_back({step, lo, hi});
+    };
+    const int64_t sa = static_cast<int64_t>(a.element_size()), sb = static_cast<int64_t>(b.element_size());
+    for (int64_t i = 0; i < a.dim(); ++i) add(a.stride(i) * sa, 0, a.size(i) - 1);
+    for (int64_t i = 0; i < b.dim(); ++i) add(b.stride(i) * sb, 1 - b.size(i), 0);
+    add(1, 1 - sb, sa - 1);
+    std::sort(terms.begin(), terms.end(), by_step);
+    int budget = kOverlapTrials;
+    return adds_up(terms.data(), terms.size(), eb.begin - ea.begin, true, budget);
+}
+
+bool same_view(const Tensor& a, const Tensor& b) {
+    return a.const_data_ptr() == b.const_data_ptr() && a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() &&
+           a.strides() == b.strides();
+}
+
 // A tensor that a call writes over: its version counts, and no element is there twice.
 void check_written(const char* op, const char* name, const Tensor& t) {
     if (t.is_inference() && !c10::InferenceMode::is_enabled())
         fail(op, std::string(name) + " is an inference tensor and can be written in inference mode only");
-    for (int64_t i = 0; i < t.dim(); ++i)
-        if (t.stride(i) == 0 && t.size(i) > 1) fail(op, std::string(name) + " has elements that share memory");
+    if (overlaps_itself(t)) fail(op, std::string(name) + " has elements that share memory");
+}
+
+// What else the call reads or writes; `own`, which each element of the written tensor is made from, may be
+// the tensor itself.
+void check_apart(const char* op, const char* name, const Tensor& t, const Tensor& own,
+                 std::initializer_list<std::pair<const char*, const Tensor*>> others) {
+    if (own.defined() && !same_view(t, own) && overlaps(t, own))
+        fail(op, std::string(name) + " shares memory with its input and is not the same view");
+    for (const auto& o : others)
+        if (o.second->defined() && overlaps(t, *o.second))
+            fail(op, std::string(name) + " shares memory with " + o.first);
 }
 
 int float_code(const char* op, const char* name, at::ScalarType t) {
@@ -295,6 +393,11 @@ PyObject* residual_norm(PyObject* const* a) {
                  w = tensor_arg(op, "weight", a[2], true), b = tensor_arg(op, "bias", a[3], true),
                  pw = tensor_arg(op, "post_weight", a[6], true), pb = tensor_arg(op, "post_bias", a[7], true),
                  gate = tensor_arg(op, "gate", a[8], true);
+    const bool inplace = bool_arg(a[12]);
+    if (inplace) {
+        check_written(op, "x", x);
+        check_apart(op, "x", x, y, {{"weight", &w}, {"bias", &b}, {"post_weight", &pw}, {"post_bias", &pb}, {"gate", &gate}});
+    }
     const int64_t dev = device_of(op, {&x, &y, &w, &b, &pw, &pb, &gate});
     const Rows r = rows_of(op, "x", x);
     m3r_residual_norm_args p = {};
@@ -333,8 +436,6 @@ PyObject* residual_norm(PyObject* const* a) {
     p.residual_scale = static_cast<float>(number_arg(op, "residual_scale", a[9]));
     p.eps = static_cast<float>(number_arg(op, "eps", a[10]));
     const at::ScalarType out_type = dtype_arg(op, a[11], (y.defined() ? y : x).scalar_type());
-    const bool inplace = bool_arg(a[12]);
-    if (inplace) check_written(op, "x", x);
     const Tensor res = inplace ? x : empty(x.sizes(), x.scalar_type(), dev);
     p.ldr = inplace ? r.ld : r.cols;
     Tensor out, scale;
@@ -388,10 +489,6 @@ PyObject* rope(PyObject* const* a) {
                  oq0 = tensor_arg(op, "out", a[8], true), ok0 = tensor_arg(op, "out", a[9], true);
     if (f.scalar_type() != at::kDouble || f.dim() != 1 || f.size(0) < 1 || (f.size(0) > 1 && f.stride(0) != 1))
         fail(op, "inv_freq must be a contiguous float64 vector");
-    const int64_t dev = device_of(op, {&q, &k, &pos, &f, &oq0, &ok0});
-    m3r_rope_args p = {};
-    p.device = static_cast<int>(dev);
-    p.dtype = float_code(op, "q", q.scalar_type());
     const bool inplace = bool_arg(a[7]);
     Tensor oq, ok;
     if (inplace) {
@@ -405,13 +502,22 @@ PyObject* rope(PyObject* const* a) {
             ok.defined() != k.defined() ||
             (k.defined() && (ok.sizes() != k.sizes() || ok.scalar_type() != k.scalar_type())))
             fail(op, "out must match q and k in shape and type");
-    } else {
+    }
+    if (oq.defined()) {
+        check_written(op, "q's result", oq);
+        if (ok.defined()) {
+            check_written(op, "k's result", ok);
+            check_apart(op, "k's result", ok, k, {{"q's result", &oq}, {"q", &q}, {"positions", &pos}, {"inv_freq", &f}});
+        }
+        check_apart(op, "q's result", oq, q, {{"k", &k}, {"positions", &pos}, {"inv_freq", &f}});
+    }
+    const int64_t dev = device_of(op, {&q, &k, &pos, &f, &oq0, &ok0});
+    m3r_rope_args p = {};
+    p.device = static_cast<int>(dev);
+    p.dtype = float_code(op, "q", q.scalar_type());
+    if (!oq.defined()) {
         oq = empty(q.sizes(), q.scalar_type(), dev);
         if (k.defined()) ok = empty(k.sizes(), k.scalar_type(), dev);
-    }
-    if (inplace || oq0.defined()) {
-        check_written(op, "q's result", oq);
-        if (ok.defined()) check_written(op, "k's result", ok);
     }
     rope_tensor(op, "q", q, oq, q, p.t[0]);
     if (k.defined()) rope_tensor(op, "k", k, ok, q, p.t[1]);

@@ -82,7 +82,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None, weight: torch.Tensor 
     groups in order (one gate for each image), or None (1).  cols is at most 16,384.
 
     Returns (r, h), h in out_dtype (default: y's type, else x's); with out_dtype torch.int8
-    (r, q, scale) as quantize_rows makes them of h.  inplace writes r over x."""
+    (r, q, scale) as quantize_rows makes them of h.  inplace writes r over x: y may be x itself then,
+    and nothing else may share memory with it."""
     return _native.residual_norm(x, y, weight, bias, norm, post_norm, post_weight, post_bias, gate, residual_scale,
                                  eps, out_dtype, inplace)
 
@@ -133,7 +134,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
 
     Strides are free apart from the last dimension's (views of a packed projection).  Returns
     (q, k) turned: new tensors, q and k themselves with inplace, or the given out = (q_out, k_out)
-    of the same shapes and type (of any strides: head-major planes for an attention kernel)."""
+    of the same shapes and type (of any strides: head-major planes for an attention kernel).  A result
+    may be its own input (the same view), and shares memory with nothing else of the call."""
     oq, ok = out if out is not None else (None, None)
     return _native.rope(q, k, positions, inv_freq, amplitude, interleaved, axes, inplace, oq, ok)
 

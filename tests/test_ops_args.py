@@ -199,3 +199,97 @@ def test_column_walk_near_the_largest_n(tmp_path):
 def test_rope_frequency_counts_that_do_not_fit_32_bits(n_freq):
     refused("m3r_rope", ROPE.pack(0, 0, 0, 1, 64, 1.0, 1, 4, 64, n_freq, 0, 0, 1, 16, 16, 16, 16, 2, 0, 128, 64, 0, 128,
                                   64, *(0,) * 9, 0), "more frequencies")
+
+
+def qkv(batch=2, tokens=5, heads=3, dim=8):
+    return torch.zeros(batch, tokens, 3, heads, dim).unbind(2)
+
+
+def rope_args(q, dim=8):
+    return torch.arange(q.shape[-3]), torch.ones(dim // 2, dtype=torch.float64)
+
+
+SHARED = "share memory|shares memory"
+
+
+def test_rope_results_that_share_memory_are_refused():
+    """A result may be its own input, and nothing else that the call reads or writes."""
+    from mast3r_runtime_b200 import ops
+
+    q, k, v = qkv()
+    flat = torch.zeros(4000)
+    freq = torch.ones(4, dtype=torch.float64)
+    pos = torch.arange(5)
+    strided = flat.as_strided((2, 5, 3, 8), (120, 20, 8, 1))  # a token's heads reach into the next token
+    for kw in (dict(q=q, k=q, inplace=True), dict(q=q, k=q[:, :, 1:], inplace=True),
+               dict(q=flat[:240].view(2, 5, 3, 8), k=flat[4:244].view(2, 5, 3, 8), inplace=True),
+               dict(q=strided, k=None, inplace=True), dict(q=q, k=None, out=(strided, None)),
+               dict(q=q, k=k, out=(v, v)), dict(q=q, k=k, out=(k, q)), dict(q=q, k=k, out=(k, v)),
+               dict(q=q, k=k, out=(v, q)), dict(q=q, k=None, out=(q.as_strided(q.shape, (24, 48, 8, 1), 200), None)),
+               dict(q=flat[:240].view(2, 5, 3, 8), k=None, out=(flat[8:248].view(2, 5, 3, 8), None)),
+               dict(q=q.expand(2, 5, 3, 8), k=None, out=(flat[:24].expand(2, 5, 24).view(2, 5, 3, 8), None))):
+        with pytest.raises(ValueError, match=SHARED):
+            ops.rope(positions=pos, inv_freq=freq, **kw)
+    whole = torch.zeros(2, 5, 3, 8)
+    for data in (torch.zeros(60, dtype=torch.int64), torch.zeros(60, dtype=torch.float64)):
+        as_float = data.view(torch.float32)
+        with pytest.raises(ValueError, match=SHARED):
+            ops.rope(as_float[:120].view(5, 3, 8), None, data[:5] if data.dtype is torch.int64 else pos,
+                     data[:4] if data.dtype is torch.float64 else freq, inplace=True)
+    # views that lie between one another without sharing an element get as far as the device
+    planes = torch.zeros(2, 3, 5, 8)
+    for kw in (dict(q=q, k=k, inplace=True), dict(q=q, k=k, out=(q, k)), dict(q=q, k=k, out=(v, k)),
+               dict(q=q, k=None, out=(v, None)), dict(q=q, k=k, out=(planes.transpose(1, 2), whole)),
+               dict(q=q[:, :, :1], k=q[:, :, 1:], inplace=True), dict(q=q[:1], k=q[1:], inplace=True),
+               dict(q=q[..., :8:1], k=None, out=(planes.transpose(1, 2), None)), dict(q=q, k=q)):
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.rope(positions=pos, inv_freq=freq, **kw)
+
+
+def test_interleaved_views_against_every_offset():
+    """The test of shared memory against a list of addresses, at every offset between two views."""
+    from mast3r_runtime_b200 import ops
+
+    flat = torch.zeros(4096)
+    freq = torch.ones(2, dtype=torch.float64)
+
+    def cells(t):
+        at = torch.tensor([t.storage_offset()])
+        for n, s in zip(t.shape, t.stride()):
+            at = (at[:, None] + torch.arange(n) * s).reshape(-1)
+        return at.tolist()
+
+    seen = {True: 0, False: 0}
+    for shape, a, b in (((2, 3, 2, 4), (60, 20, 8, 1), (60, 20, 8, 1)), ((2, 3, 2, 4), (60, 20, 8, 1), (40, 8, 20, 1)),
+                        ((3, 2, 2, 4), (7, 24, 60, 1), (7, 24, 60, 1)), ((2, 3, 2, 4), (4, 16, 8, 1), (48, 8, 4, 1)),
+                        ((1, 4, 3, 4), (0, 12, 4, 1), (0, 5, 24, 1)), ((2, 2, 2, 4), (64, 16, 32, 1), (64, 16, 32, 1)),
+                        ((2, 2, 2, 4), (64, 16, 32, 1), (32, 64, 16, 1))):
+        for off in range(0, 130):
+            x, y = flat.as_strided(shape, a, 70), flat.as_strided(shape, b, off)
+            twice = any(len(set(cells(t))) != len(cells(t)) for t in (x, y))
+            same = off == 70 and a == b
+            shared = twice or bool(set(cells(x)) & set(cells(y)))
+            with pytest.raises(ValueError, match=SHARED if shared else "CUDA"):
+                ops.rope(x, y, torch.arange(shape[1]), freq, inplace=True)
+            if not same:
+                with pytest.raises(ValueError, match=SHARED if shared else "CUDA"):
+                    ops.rope(x, None, torch.arange(shape[1]), freq, out=(y, None))
+            seen[shared] += 1
+    assert min(seen.values()) > 40  # both answers are well covered
+
+
+def test_residual_norm_in_place_over_its_inputs_is_refused():
+    from mast3r_runtime_b200 import ops
+
+    flat = torch.zeros(400)
+    x = flat[40:360].view(10, 32)
+    for kw in (dict(y=flat[8:328].view(10, 32)), dict(y=x.flip(0), weight=x[3]), dict(y=x, gate=x[9]),
+               dict(y=None, bias=flat[30:62]), dict(y=x, post_norm="rms", post_weight=x[0]),
+               dict(y=x, post_norm="rms", post_bias=flat[350:382]), dict(y=x.new_zeros(10, 32), gate=x[:2])):
+        with pytest.raises(ValueError, match=SHARED):
+            ops.residual_norm(x, kw.pop("y"), kw.pop("weight", None), inplace=True, **kw)
+    wide = torch.zeros(10, 96)
+    for kw in (dict(x=x, y=x), dict(x=x, y=None, weight=flat[:32]), dict(x=wide[:, :32], y=wide[:, 32:64]),
+               dict(x=wide[:, 8:40], y=wide[:, 40:72], weight=wide[0, 72:].repeat(2)[:32])):
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.residual_norm(kw.pop("x"), kw.pop("y"), kw.pop("weight", None), inplace=True, **kw)
