@@ -7,6 +7,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAStream.h>
@@ -49,15 +50,22 @@ Tensor tensor_arg(const char* op, const char* name, PyObject* o, bool none = fal
     fail(op, std::string(name) + " must be a tensor" + (none ? " or None" : ""));
 }
 
+// The device of a call's tensors.  No gradient is computed, in either mode of differentiation.
 int64_t device_of(const char* op, std::initializer_list<const Tensor*> all) {
     int64_t dev = -1;
     const bool grad = c10::GradMode::is_enabled();
+    const bool tangent = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Tensor* t : all) {
+        if (!t->defined()) continue;
+        if (grad && t->requires_grad()) fail(op, "no gradient is computed (use torch.no_grad() or detach the tensors)");
+        if (tangent && t->_fw_grad(0).defined())
+            fail(op, "no forward-mode gradient is computed (pass the primal: torch.autograd.forward_ad.unpack_dual)");
+    }
     for (const Tensor* t : all) {
         if (!t->defined()) continue;
         if (!t->is_cuda()) fail(op, "tensors must be on a CUDA device");
         if (dev < 0) dev = t->get_device();
         if (t->get_device() != dev) fail(op, "tensors are on different devices");
-        if (grad && t->requires_grad()) fail(op, "no gradient is computed (use torch.no_grad() or detach the tensors)");
     }
     return dev;
 }

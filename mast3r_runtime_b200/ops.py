@@ -14,7 +14,7 @@ results and workspace come from torch's allocator.  All tensors of a call are on
 last dimension of the large ones is contiguous (other strides are free).  Bad arguments raise
 ValueError before anything is launched, device errors RuntimeError.  The operators have no
 gradients: the package runs models, it does not train them, and a call with a tensor that requires
-grad outside torch.no_grad() is refused.
+grad outside torch.no_grad(), or with one that carries a forward-mode tangent, is refused.
 """
 
 from __future__ import annotations

@@ -293,3 +293,29 @@ def test_residual_norm_in_place_over_its_inputs_is_refused():
                dict(x=wide[:, 8:40], y=wide[:, 40:72], weight=wide[0, 72:].repeat(2)[:32])):
         with pytest.raises(ValueError, match="CUDA"):
             ops.residual_norm(kw.pop("x"), kw.pop("y"), kw.pop("weight", None), inplace=True, **kw)
+
+
+def test_tangents_are_refused():
+    """A forward-mode derivative would be dropped; without forward mode the value alone is used."""
+    import torch.autograd.forward_ad as fwd
+
+    from mast3r_runtime_b200 import ops
+
+    x, w, ws = torch.zeros(4, 32), torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8)
+    q, pos, f = x.view(4, 1, 32), torch.arange(4), torch.ones(16, dtype=torch.float64)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: ops.quantize_rows(dual(x)), lambda: ops.int8_linear(dual(x), w, ws),
+                     lambda: ops.int8_linear(x, w, ws, dual(ws)), lambda: ops.residual_norm(x, dual(x), None),
+                     lambda: ops.residual_norm(x, x, None, gate=dual(x[0])), lambda: ops.rope(dual(q), None, pos, f),
+                     lambda: ops.rope(q, q.clone(), pos, dual(f)), lambda: ops.quantize_weight(dual(x))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+                call()
+            with torch.inference_mode(), pytest.raises(ValueError, match="CUDA"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.quantize_rows(x)
