@@ -44,6 +44,8 @@ Tensor tensor_arg(const char* op, const char* name, PyObject* o, bool none = fal
     if (THPVariable_Check(o)) {
         const Tensor& t = THPVariable_Unpack(o);
         if (t.layout() != at::kStrided) fail(op, std::string(name) + " must be a dense tensor");
+        if (t.is_neg() || t._is_zerotensor())
+            fail(op, std::string(name) + " does not hold its values in memory (use resolve_neg() or clone())");
         return t;
     }
     if (none && o == Py_None) return Tensor();

@@ -319,3 +319,23 @@ def test_tangents_are_refused():
                 call()
         with pytest.raises(ValueError, match="CUDA"):
             ops.quantize_rows(x)
+
+
+def test_tensors_whose_memory_is_not_their_values_are_refused():
+    """The imaginary part of a conjugate is its memory with the sign still to change; a tensor of
+    symbolic zeros has no memory."""
+    from mast3r_runtime_b200 import ops
+
+    lazy = torch.zeros(4, 32, dtype=torch.complex64).conj().imag
+    assert lazy.is_neg()
+    zero = torch._efficientzerotensor(4, 32)
+    x, w, ws = torch.zeros(4, 32), torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8)
+    pos, f = torch.arange(4), torch.ones(16, dtype=torch.float64)
+    for t in (lazy, zero):
+        for call in (lambda: ops.quantize_rows(t), lambda: ops.int8_linear(t, w, ws),
+                     lambda: ops.residual_norm(x, t, None), lambda: ops.residual_norm(t, None, None, inplace=True),
+                     lambda: ops.residual_norm(x, x, t[0]), lambda: ops.rope(t.view(4, 1, 32), None, pos, f)):
+            with pytest.raises(ValueError, match="values in memory"):
+                call()
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.quantize_rows(lazy.resolve_neg())
