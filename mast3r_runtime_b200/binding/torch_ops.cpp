@@ -201,7 +201,14 @@ double number_arg(const char* op, const char* name, PyObject* o) {
     return v;
 }
 
-bool bool_arg(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool bool_arg(const char* op, const char* name, PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        fail(op, std::string(name) + " must be true or false");
+    }
+    return v == 1;
+}
 
 // One of the names in `names` (its index), or `none` for None where that is allowed.
 int name_arg(const char* op, const char* what, PyObject* o, std::initializer_list<const char*> names, int none = -1) {
@@ -403,7 +410,7 @@ PyObject* residual_norm(PyObject* const* a) {
                  w = tensor_arg(op, "weight", a[2], true), b = tensor_arg(op, "bias", a[3], true),
                  pw = tensor_arg(op, "post_weight", a[6], true), pb = tensor_arg(op, "post_bias", a[7], true),
                  gate = tensor_arg(op, "gate", a[8], true);
-    const bool inplace = bool_arg(a[12]);
+    const bool inplace = bool_arg(op, "inplace", a[12]);
     if (inplace) {
         check_written(op, "x", x);
         check_apart(op, "x", x, y, {{"weight", &w}, {"bias", &b}, {"post_weight", &pw}, {"post_bias", &pb}, {"gate", &gate}});
@@ -499,7 +506,7 @@ PyObject* rope(PyObject* const* a) {
                  oq0 = tensor_arg(op, "out", a[8], true), ok0 = tensor_arg(op, "out", a[9], true);
     if (f.scalar_type() != at::kDouble || f.dim() != 1 || f.size(0) < 1 || (f.size(0) > 1 && f.stride(0) != 1))
         fail(op, "inv_freq must be a contiguous float64 vector");
-    const bool inplace = bool_arg(a[7]);
+    const bool inplace = bool_arg(op, "inplace", a[7]), interleaved = bool_arg(op, "interleaved", a[5]);
     Tensor oq, ok;
     if (inplace) {
         if (oq0.defined() || ok0.defined()) fail(op, "inplace and out exclude each other");
@@ -537,7 +544,7 @@ PyObject* rope(PyObject* const* a) {
     p.dim = q.size(d - 1);
     p.n_freq = f.size(0);
     p.amplitude = static_cast<float>(number_arg(op, "amplitude", a[4]));
-    p.interleaved = bool_arg(a[5]);
+    p.interleaved = interleaved;
     const double axes = number_arg(op, "axes", a[6]);
     if (axes != 1 && axes != 2) fail(op, "axes must be 1 or 2");
     p.axes = static_cast<int>(axes);

@@ -339,3 +339,17 @@ def test_tensors_whose_memory_is_not_their_values_are_refused():
                 call()
     with pytest.raises(ValueError, match="CUDA"):
         ops.quantize_rows(lazy.resolve_neg())
+
+
+@pytest.mark.parametrize("flag", [torch.zeros(2), "meta"])
+def test_flags_without_a_truth_value_are_refused(flag):
+    from mast3r_runtime_b200 import ops
+
+    if flag == "meta":
+        flag = torch.zeros((), device="meta")
+    x = torch.zeros(4, 1, 32)
+    with pytest.raises(ValueError, match="true or false"):
+        ops.residual_norm(x[:, 0], x[:, 0], None, inplace=flag)
+    for kw in (dict(inplace=flag), dict(interleaved=flag)):
+        with pytest.raises(ValueError, match="true or false"):
+            ops.rope(x, None, torch.arange(4), torch.ones(16, dtype=torch.float64), **kw)
