@@ -25,11 +25,13 @@ void allow_smem(Kernel kern, int bytes, unsigned& done) {
 // A launch that may start before the kernel ahead of it on the stream has finished (the kernel keeps the
 // rules of common.cuh: grid_dependency_wait before it touches memory, plain loads), which hides its start
 // behind that one's end (24 x 4,096 x 4,096 with its quantisation, one call after the other: 10.2 us
-// against 8.4); cluster size 0: none.
+// against 8.4); cluster size 0: none.  With `dependent` false, an ordinary launch.  Launched with
+// cudaLaunchKernelEx either way, whose status is this launch's own: cudaGetLastError would also give an error
+// that an earlier call of the thread left.
 struct LaunchConfig {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    LaunchConfig(unsigned grid, int block, int smem, cudaStream_t s, int cluster = 0) {
+    LaunchConfig(unsigned grid, int block, int smem, cudaStream_t s, int cluster = 0, bool dependent = true) {
         cfg.gridDim = dim3(grid);
         cfg.blockDim = dim3(block);
         cfg.dynamicSmemBytes = smem;
@@ -41,7 +43,7 @@ struct LaunchConfig {
         attr[1].val.clusterDim.y = 1;
         attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = cluster > 0 ? 2 : 1;
+        cfg.numAttrs = cluster > 0 ? 2 : dependent ? 1 : 0;
     }
     LaunchConfig(const LaunchConfig&) = delete;
 };

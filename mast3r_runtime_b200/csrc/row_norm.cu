@@ -437,8 +437,8 @@ void launch(cudaStream_t s, const RowNormParams& p, int threads) {
         } else {
             // an ordinary launch: it reads the weight vectors as constants (__ldg), which may come from the
             // kernel before (40,001 rows of 129: 21 us against 27 with plain loads)
-            row_norm_kernel<VEC, NCH, LANES, ROW_FULL, GT><<<static_cast<unsigned>(grid), threads, 0, s>>>(p);
-            M3R_CUDA(cudaGetLastError());
+            const LaunchConfig plain(static_cast<unsigned>(grid), threads, 0, s, 0, false);
+            M3R_CUDA(cudaLaunchKernelEx(&plain.cfg, row_norm_kernel<VEC, NCH, LANES, ROW_FULL, GT>, p));
         }
         return;
     }
@@ -460,8 +460,8 @@ bool launch_stream(cudaStream_t s, const RowNormParams& p, int threads) {
     if (stages < 1) return false;
     static unsigned done = 0;
     allow_smem(row_stream_kernel, kMost, done);
-    row_stream_kernel<<<148 * per_sm, threads, stages * row, s>>>(p, stages);
-    M3R_CUDA(cudaGetLastError());
+    const LaunchConfig c(static_cast<unsigned>(148 * per_sm), threads, stages * row, s, 0, false);
+    M3R_CUDA(cudaLaunchKernelEx(&c.cfg, row_stream_kernel, p, stages));
     return true;
 }
 

@@ -1,5 +1,5 @@
 """GPU tests of the operators at the edges of their ranges: results far below the values they are
-made from, columns that are not finite.
+made from, columns that are not finite, errors of one call that must not show in the next.
 
 Tolerances count roundings as test_gpu_ops.py does: U = 2^-24 is one 32-bit rounding, half(dtype)
 half a step of the result's type."""
@@ -13,7 +13,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_ops import DT, U, close, half, ops  # noqa: E402,F401
+from test_gpu_ops import DT, U, close, half, ops, residual64, rnd  # noqa: E402,F401
 
 
 # ----------------------------------------------------------------------------- GELU
@@ -69,3 +69,36 @@ def test_gelu_columns_that_are_not_finite_stay_alone(ops, m, n, out):  # noqa: F
     assert torch.isnan(z[:, 5]).all()
     up = q[:, 0] > 0
     assert torch.isposinf(z[up, 18]).all() and torch.isnan(z[~up, 18]).all()
+
+
+# ----------------------------------------------------------------------------- errors
+@pytest.mark.skipif("torch.cuda.device_count() >= 8")
+def test_an_error_of_one_call_does_not_show_in_the_next(ops):  # noqa: F811
+    """A device that does not exist fails that call alone."""
+    from test_ops_args import QUANTIZE, RESIDUAL
+
+    from mast3r_runtime_b200 import _lib
+
+    lib = _lib.load()
+    x, gate = rnd(6, 41, seed=1), rnd(41, seed=2)
+    r, h = torch.empty_like(x), torch.empty_like(x)
+    q, s = torch.empty(6, 48, dtype=torch.int8, device="cuda"), torch.empty(6, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    none = torch.cuda.device_count()  # the first that does not exist
+    args = RESIDUAL.pack(0, 2, 2, 2, 1, 0, 1e-6, 1.0, 6, 41, 41, 41, 41, 41, 0, 0, x.data_ptr(), x.data_ptr(),
+                         gate.data_ptr(), 0, 0, 0, 0, r.data_ptr(), h.data_ptr(), 0, stream)
+    bad = QUANTIZE.pack(none, 2, 6, 41, 41, 48, x.data_ptr(), q.data_ptr(), s.data_ptr(), 0)
+    for _ in range(2):
+        assert lib.m3r_quantize_rows(bad) == -3 and lib.m3r_global_error()
+        assert lib.m3r_residual_norm(args) == 0, lib.m3r_global_error()
+        want = residual64(x, x, gate, 1.0, None, None, None)
+        close(r, *want)
+    # nor does the engine's next launch see it
+    from test_gpu_failure import _attention_ok
+
+    assert lib.m3r_quantize_rows(bad) == -3 and _attention_ok(lib)
+    # an error that another entry point left behind stays its own too
+    d = torch.zeros(300, 24, device="cuda")
+    nn = torch.empty(300, dtype=torch.int32, device="cuda")
+    assert lib.m3r_match_nn_static(none, d.data_ptr(), d.data_ptr(), 300, 300, 24, nn.data_ptr(), nn.data_ptr(), 0, 0) != 0
+    assert lib.m3r_residual_norm(args) == 0, lib.m3r_global_error()
