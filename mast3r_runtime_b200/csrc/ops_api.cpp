@@ -50,6 +50,10 @@ struct OpDevice {
     }
 };
 
+void check_device(const char* op, int dev) {
+    M3R_REQUIRE(dev >= 0 && dev < M3R_MAX_DEVICES, std::string(op) + ": bad device");
+}
+
 bool is_float(int dt) { return dt == M3R_DTYPE_BF16 || dt == M3R_DTYPE_F16 || dt == M3R_DTYPE_F32; }
 
 // `p` is aligned to its elements
@@ -95,6 +99,7 @@ extern "C" {
 int m3r_quantize_rows(const m3r_quantize_args* args) {
     return guarded([&] {
         M3R_REQUIRE(args != nullptr, "quantize_rows: null arguments");
+        check_device("quantize_rows", args->device);
         const m3r::RowNormParams p = quantize_params(*args);
         OpDevice g(args->device);
         m3r::row_norm(static_cast<cudaStream_t>(args->stream), p);
@@ -117,6 +122,7 @@ int64_t m3r_int8_linear_workspace(int x_dtype, int64_t rows, int64_t n, int64_t 
 int m3r_int8_linear(const m3r_int8_linear_args* args) {
     return guarded([&] {
         M3R_REQUIRE(args != nullptr, "int8_linear: null arguments");
+        check_device("int8_linear", args->device);
         const m3r_int8_linear_args& a = *args;
         M3R_REQUIRE(is_float(a.x_dtype) || a.x_dtype == M3R_DTYPE_I8, "int8_linear: x must be bf16, fp16, fp32 or int8");
         M3R_REQUIRE(is_float(a.out_dtype), "int8_linear: the output must be bf16, fp16 or fp32");
@@ -171,6 +177,7 @@ int m3r_int8_linear(const m3r_int8_linear_args* args) {
 int m3r_residual_norm(const m3r_residual_norm_args* args) {
     return guarded([&] {
         M3R_REQUIRE(args != nullptr, "residual_norm: null arguments");
+        check_device("residual_norm", args->device);
         const m3r_residual_norm_args& a = *args;
         check_rows("residual_norm", a.rows, a.cols);
         M3R_REQUIRE(is_float(a.x_dtype), "residual_norm: x must be bf16, fp16 or fp32");
@@ -238,6 +245,7 @@ int m3r_residual_norm(const m3r_residual_norm_args* args) {
 int m3r_rope(const m3r_rope_args* args) {
     return guarded([&] {
         M3R_REQUIRE(args != nullptr, "rope: null arguments");
+        check_device("rope", args->device);
         const m3r_rope_args& a = *args;
         M3R_REQUIRE(is_float(a.dtype), "rope: values must be bf16, fp16 or fp32");
         M3R_REQUIRE(a.axes == 1 || a.axes == 2, "rope: axes must be 1 or 2");
@@ -298,6 +306,7 @@ int m3r_rope(const m3r_rope_args* args) {
 
 int m3r_operator_status(int device, void* stream) {
     return guarded([&] {
+        check_device("operator_status", device);
         OpDevice g(device);
         const int product = m3r::int8_linear_status(static_cast<cudaStream_t>(stream));
         const int rows = m3r::row_norm_status(static_cast<cudaStream_t>(stream));

@@ -353,3 +353,17 @@ def test_flags_without_a_truth_value_are_refused(flag):
     for kw in (dict(inplace=flag), dict(interleaved=flag)):
         with pytest.raises(ValueError, match="true or false"):
             ops.rope(x, None, torch.arange(4), torch.ones(16, dtype=torch.float64), **kw)
+
+
+@pytest.mark.parametrize("device", [-1, 16, 2 ** 31 - 1])
+def test_device_numbers_out_of_range_are_bad_arguments(device):
+    refused("m3r_quantize_rows", QUANTIZE.pack(device, 0, 2, 8, 8, 16, 16, 16, 16, 0), "device")
+    refused("m3r_int8_linear", LINEAR.pack(device, 3, 1, 0, 4, 32, 64, 64, 64, 32, 256, 256, 256, 256, 0, 256, 0, 0, 0),
+            "device")
+    refused("m3r_residual_norm", RESIDUAL.pack(device, 2, 0, 0, 1, 0, 1e-6, 1.0, 4, 8, 8, 8, 8, 8, 0, 0, 16, 16, 0, 0, 0,
+                                               16, 16, 32, 16, 0, 0), "device")
+    refused("m3r_rope", ROPE.pack(device, 0, 0, 1, 64, 1.0, 1, 4, 64, 32, 0, 0, 1, 16, 16, 16, 16, 2, 0, 128, 64, 0, 128,
+                                  64, *(0,) * 9, 0), "device")
+    from mast3r_runtime_b200 import _lib
+
+    assert _lib.load().m3r_operator_status(device, None) == -1
