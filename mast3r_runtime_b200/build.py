@@ -5,7 +5,8 @@
 Objects go to mast3r_runtime_b200/_build/ (rebuilt when a source or header is newer);
 the shared libraries are written next to this file so that they travel with the tree.
 _torch_ops.so (binding/torch_ops.cpp, the tensors of mast3r_runtime_b200.ops) is built against the
-torch of this interpreter, and left out where there is none: nothing else in the package needs it.
+torch of this interpreter, and left out where that is not there, has no CUDA or no headers: nothing else
+in the package needs it.
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ LIB = HERE / "libm3r_cuda.so"
 INCLUDE = HERE.parent / "include"
 BINDING = HERE / "binding" / "torch_ops.cpp"
 TORCH_LIB = HERE / "_torch_ops.so"
+TORCH_STAMP = HERE / "_torch_ops.stamp"  # what it was built for; travels with it
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -77,22 +79,39 @@ def build(verbose: bool = False) -> Path:
     if verbose:
         print(f"built {LIB}")
     binding = build_torch_ops()
-    if verbose:
-        print(f"built {binding}" if binding else "no torch: mast3r_runtime_b200.ops is not built")
+    if verbose and binding:
+        print(f"built {binding}")
     return LIB
 
 
+def _missing_for_torch_ops(torch: Path | None) -> str | None:
+    """What the binding needs and this interpreter does not have."""
+    if torch is None:
+        return "no torch"
+    for lib in ("libtorch_python.so", "libtorch_cuda.so", "libc10_cuda.so"):
+        if not (torch / "lib" / lib).exists():
+            return f"torch without {lib}"
+    if not (torch / "include" / "ATen" / "ATen.h").exists():
+        return "torch without headers"
+    if not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        return "no Python headers"
+    return None
+
+
 def build_torch_ops() -> Path | None:
-    """_torch_ops.so, rebuilt when its source, the C header or torch's version changed."""
+    """_torch_ops.so, rebuilt when its source, the C header, torch's or Python's version changed; None
+    where it is left out."""
     spec = importlib.util.find_spec("torch")
-    if spec is None:
+    root = Path(spec.origin).parent if spec is not None and spec.origin else None
+    missing = _missing_for_torch_ops(root)
+    if missing:
+        print(f"{missing}: mast3r_runtime_b200.ops is not built", file=sys.stderr)
+        TORCH_LIB.unlink(missing_ok=True)
         return None
-    root = Path(spec.origin).parent
-    version = (root / "version.py").read_text()
-    stamp = BUILD / "torch_ops.version"
+    version = (root / "version.py").read_text() + f"python {sysconfig.get_config_var('SOABI')}\n"
     newest = max(BINDING.stat().st_mtime, (INCLUDE / "m3r_cuda.h").stat().st_mtime)
-    if TORCH_LIB.exists() and TORCH_LIB.stat().st_mtime >= newest and (
-            not stamp.exists() or stamp.read_text() == version):
+    if (TORCH_LIB.exists() and TORCH_LIB.stat().st_mtime >= newest and TORCH_STAMP.exists()
+            and TORCH_STAMP.read_text() == version):
         return TORCH_LIB
     cuda = Path(nvcc()).resolve().parent.parent / "include"
     tmp = BUILD / TORCH_LIB.name
@@ -105,7 +124,7 @@ def build_torch_ops() -> Path | None:
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for {BINDING.name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, TORCH_LIB)
-    stamp.write_text(version)
+    TORCH_STAMP.write_text(version)
     return TORCH_LIB
 
 
