@@ -403,6 +403,10 @@ int m3r_rope(const m3r_rope_args* args);
  * (M3R_ERR_TIMEOUT; the outputs of the calls since are undefined, the context stays usable).
  * Not to be called during a stream capture. */
 int m3r_operator_status(int device, void* stream);
+/* Queues a kernel that waits limit_ns (up to 10 s) for a signal that nothing sends, as the product's
+ * kernels (which = 0) or the row kernels (1) would: the next m3r_operator_status reports it.  For tests
+ * of a caller's failure path. */
+int m3r_operator_wait_selftest(int device, int which, unsigned long long limit_ns, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

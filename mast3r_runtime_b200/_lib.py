@@ -112,6 +112,7 @@ SIGNATURES = {
     "m3r_residual_norm": (_I, [_P]),
     "m3r_rope": (_I, [_P]),
     "m3r_operator_status": (_I, [_I, _P]),
+    "m3r_operator_wait_selftest": (_I, [_I, _I, ctypes.c_ulonglong, _P]),
     "m3r_check_checkpoint": (_I, [ctypes.POINTER(M3RConfig), ctypes.c_char_p]),
 }
 

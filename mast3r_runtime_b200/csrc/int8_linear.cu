@@ -683,15 +683,10 @@ void int8_linear(cudaStream_t s, const Int8LinearParams& p) {
         launch<64, 1>(s, p, xq, ldq, xs, sms);
 }
 
-int int8_linear_status(cudaStream_t s) {
-    DevStatus st;
-    M3R_CUDA(cudaStreamSynchronize(s));
-    M3R_CUDA(cudaMemcpyFromSymbol(&st, g_status, sizeof(st)));
-    if (st.code != 0) {
-        const DevStatus zero = {};
-        M3R_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
-    }
-    return st.code;
+int* int8_linear_status() {
+    void* at = nullptr;
+    M3R_CUDA(cudaGetSymbolAddress(&at, g_status));
+    return &static_cast<DevStatus*>(at)->code;
 }
 
 }  // namespace m3r

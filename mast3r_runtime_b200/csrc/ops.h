@@ -38,9 +38,9 @@ struct RowNormParams {
     float* out_scale;   // rows of an 8-bit result
 };
 void row_norm(cudaStream_t s, const RowNormParams& p);
-// Code of the first device wait of a row kernel that ran out on the current device (0: none), read
-// after the stream's work; clears it.
-int row_norm_status(cudaStream_t s);
+// Device address of the code that the first wait of a row kernel to run out on the current device leaves
+// (0: none).
+int* row_norm_status();
 
 // Rotary positions on up to two tensors [batch, tokens, heads, dim].
 struct RopeTensor {
@@ -78,6 +78,10 @@ struct Int8LinearParams {
 size_t int8_linear_workspace(int x_dt, long long rows, int n, int k);
 void int8_linear(cudaStream_t s, const Int8LinearParams& p);
 // The same for the product's kernels.
-int int8_linear_status(cudaStream_t s);
+int* int8_linear_status();
+
+// selftest.cu: queues one warp that waits `limit_ns` for a signal that nothing sends and leaves the code of
+// that at `status`, where it is 0.
+void run_out_wait(cudaStream_t s, int* status, unsigned long long limit_ns);
 
 }  // namespace m3r

@@ -308,10 +308,29 @@ int m3r_operator_status(int device, void* stream) {
     return guarded([&] {
         check_device("operator_status", device);
         OpDevice g(device);
-        const int product = m3r::int8_linear_status(static_cast<cudaStream_t>(stream));
-        const int rows = m3r::row_norm_status(static_cast<cudaStream_t>(stream));
-        const int code = product ? product : rows;
-        if (code) throw m3r::Error(m3r::kErrTimeout, "device wait timed out (code " + std::to_string(code) + ")");
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        int first = 0;
+        for (int* at : {m3r::int8_linear_status(), m3r::row_norm_status()}) {
+            int code = 0;
+            M3R_CUDA(cudaMemcpyAsync(&code, at, sizeof(code), cudaMemcpyDeviceToHost, s));
+            M3R_CUDA(cudaStreamSynchronize(s));
+            if (code == 0) continue;
+            M3R_CUDA(cudaMemsetAsync(at, 0, sizeof(code), s));  // the code alone, and before this returns
+            M3R_CUDA(cudaStreamSynchronize(s));
+            if (first == 0) first = code;
+        }
+        if (first) throw m3r::Error(m3r::kErrTimeout, "device wait timed out (code " + std::to_string(first) + ")");
+    });
+}
+
+int m3r_operator_wait_selftest(int device, int which, unsigned long long limit_ns, void* stream) {
+    return guarded([&] {
+        check_device("operator_wait_selftest", device);
+        M3R_REQUIRE(which == 0 || which == 1, "operator_wait_selftest: unknown group of kernels");
+        M3R_REQUIRE(limit_ns > 0 && limit_ns <= 10000000000ull, "operator_wait_selftest: limit must be in (0, 10 s]");
+        OpDevice g(device);
+        m3r::run_out_wait(static_cast<cudaStream_t>(stream), which == 0 ? m3r::int8_linear_status() : m3r::row_norm_status(),
+                          limit_ns);
     });
 }
 

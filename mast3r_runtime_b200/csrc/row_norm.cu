@@ -527,15 +527,10 @@ void dispatch_elements(cudaStream_t s, const RowNormParams& p) {
 
 }  // namespace
 
-int row_norm_status(cudaStream_t s) {
-    DevStatus st;
-    M3R_CUDA(cudaStreamSynchronize(s));
-    M3R_CUDA(cudaMemcpyFromSymbol(&st, g_status, sizeof(st)));
-    if (st.code != 0) {
-        const DevStatus zero = {};
-        M3R_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
-    }
-    return st.code;
+int* row_norm_status() {
+    void* at = nullptr;
+    M3R_CUDA(cudaGetSymbolAddress(&at, g_status));
+    return &static_cast<DevStatus*>(at)->code;
 }
 
 void row_norm(cudaStream_t s, const RowNormParams& p) {

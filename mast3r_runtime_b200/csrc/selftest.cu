@@ -9,6 +9,8 @@
 #include "../../include/m3r_cuda.h"
 #include "common.cuh"
 #include "engine.h"
+#include "launch.h"
+#include "ops.h"
 #include "tmap.h"
 
 namespace m3r {
@@ -30,7 +32,33 @@ __global__ void never_signalled_wait_kernel(int* status) {
     __syncthreads();
 }
 
+// The same with the limit and the status block of this launch alone, so that the limit of other launches
+// is left as it is; the code goes to `status`.
+__global__ void run_out_wait_kernel(int* status, unsigned long long limit_ns) {
+    __shared__ uint64_t bar;
+    __shared__ int abort_flag;
+    __shared__ m3r::DevStatus own;
+    if (threadIdx.x == 0) {
+        m3r::mbar_init(&bar, 1);
+        abort_flag = 0;
+        own = {0, 0, limit_ns};
+        m3r::fence_barrier_init();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && !m3r::mbar_wait(&bar, 0, &abort_flag, m3r::kDevTimeoutMma, &own.code)) {
+        const int code = own.code;
+        atomicCAS(status, 0, code);
+    }
+}
+
 }  // namespace
+
+namespace m3r {
+void run_out_wait(cudaStream_t s, int* status, unsigned long long limit_ns) {
+    const LaunchConfig c(1, 32, 0, s, 0, false);
+    M3R_CUDA(cudaLaunchKernelEx(&c.cfg, run_out_wait_kernel, status, limit_ns));
+}
+}  // namespace m3r
 
 extern "C" {
 

@@ -102,3 +102,35 @@ def test_an_error_of_one_call_does_not_show_in_the_next(ops):  # noqa: F811
     nn = torch.empty(300, dtype=torch.int32, device="cuda")
     assert lib.m3r_match_nn_static(none, d.data_ptr(), d.data_ptr(), 300, 300, 24, nn.data_ptr(), nn.data_ptr(), 0, 0) != 0
     assert lib.m3r_residual_norm(args) == 0, lib.m3r_global_error()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_wait_that_ran_out_is_reported_once(ops, which):  # noqa: F811
+    """The product's kernels and the row kernels each record it; the next calls are sound."""
+    from mast3r_runtime_b200 import _lib
+
+    lib = _lib.load()
+    ops.status(0)
+    side = torch.cuda.Stream()
+    for stream, limit in ((torch.cuda.current_stream(), 1_000_000), (side, 3_000_000)):
+        assert lib.m3r_operator_wait_selftest(0, which, limit, stream.cuda_stream) == 0, lib.m3r_global_error()
+        with torch.cuda.stream(stream):
+            with pytest.raises(RuntimeError, match="timed out"):
+                ops.status(0)
+            ops.status(0)
+            q, w, ws = gelu_inputs(200, 40)
+            y = ops.int8_linear(q, w, ws, x_scale=torch.ones(200, device="cuda"), out_dtype=torch.float32)
+            v = q[:, :1].double() * 127 * ws.double()
+            close(y, v, 4 * U * v.abs())
+            x = rnd(3000, 1024, seed=3)
+            r, _ = ops.residual_norm(x, x, None)
+            assert torch.equal(r, x + x)
+            ops.status(0)
+
+
+def test_wait_selftest_refusals(ops):  # noqa: F811
+    from mast3r_runtime_b200 import _lib
+
+    lib = _lib.load()
+    for args in ((0, 2, 1000), (0, -1, 1000), (0, 0, 0), (0, 0, 20_000_000_000), (-1, 0, 1000)):
+        assert lib.m3r_operator_wait_selftest(*args, None) == -1
