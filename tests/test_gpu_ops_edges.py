@@ -1,5 +1,6 @@
 """GPU tests of the operators at the edges of their ranges: results far below the values they are
-made from, columns that are not finite, errors of one call that must not show in the next.
+made from, columns and rows that are not finite, heads and head
+counts past a block's share, errors of one call that must not show in the next.
 
 Tolerances count roundings as test_gpu_ops.py does: U = 2^-24 is one 32-bit rounding, half(dtype)
 half a step of the result's type."""
@@ -13,7 +14,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_ops import DT, U, close, half, ops, residual64, rnd  # noqa: E402,F401
+from test_gpu_ops import DT, U, close, half, ops, residual64, rnd, rope64  # noqa: E402,F401
 
 
 # ----------------------------------------------------------------------------- GELU
@@ -134,3 +135,56 @@ def test_wait_selftest_refusals(ops):  # noqa: F811
     lib = _lib.load()
     for args in ((0, 2, 1000), (0, -1, 1000), (0, 0, 0), (0, 0, 20_000_000_000), (-1, 0, 1000)):
         assert lib.m3r_operator_wait_selftest(*args, None) == -1
+
+
+# ----------------------------------------------------------------------------- rope
+@pytest.mark.parametrize("dim,rot,dtype", [(4096, 4096, "fp32"), (4096, 2400, "bf16"), (1400, 1400, "fp32"),
+                                           (1030, 1026, "fp16")])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_heads_longer_than_a_block(ops, dim, rot, dtype, interleaved):  # noqa: F811
+    """Heads with more accesses than a block has threads."""
+    f, amp = ops.rope_frequencies(rot)
+    for t, h, kv in ((1, 1, 1), (5, 3, 1)):
+        q, k = rnd(1, t, h, dim, seed=1, dtype=DT[dtype]), rnd(1, t, kv, dim, seed=2, dtype=DT[dtype])
+        pos = torch.arange(t, device="cuda") * 117 + 3
+        for x, o in zip((q, k), ops.rope(q, k, pos, f, interleaved=interleaved)):
+            want, tol = rope64(x, pos[None, None], f, 1.0, interleaved, 1)
+            close(o, want, tol)
+
+
+@pytest.mark.parametrize("tokens", [1, 700])
+@pytest.mark.parametrize("heads,kv", [(300, 100), (257, 1), (1, 600), (512, 512)])
+def test_rope_more_heads_than_a_block_takes(ops, tokens, heads, kv):  # noqa: F811
+    f, _ = ops.rope_frequencies(16)
+    q, k = rnd(1, tokens, heads, 24, seed=1), rnd(1, tokens, kv, 24, seed=2)
+    pos = torch.arange(tokens, device="cuda") - 5
+    for x, o in zip((q, k), ops.rope(q, k, pos, f)):
+        want, tol = rope64(x, pos[None, None], f, 1.0, False, 1)
+        close(o, want, tol)
+
+
+# ----------------------------------------------------------------------------- residual_norm
+@pytest.mark.parametrize("rows,cols", [(9, 24), (9, 1024), (9, 1001), (3000, 1024), (9, 5003), (700, 4096)])
+@pytest.mark.parametrize("norm,post", [("layer", None), ("rms", "layer")])
+def test_residual_norm_rows_that_are_not_finite_stay_alone(ops, rows, cols, norm, post):  # noqa: F811
+    x, y = rnd(rows, cols, seed=1), rnd(rows, cols, seed=2, dtype=torch.bfloat16)
+    w = 1 + 0.1 * rnd(cols, seed=3)
+    kw = dict(norm=norm, post_norm=post)
+    r, h = ops.residual_norm(x, y, w, out_dtype=torch.float32, **kw)
+    x2, y2 = x.clone(), y.clone()
+    x2[1, 3], x2[4, cols - 1], y2[6, 0], y2[8, cols // 2] = math.inf, math.nan, -math.inf, math.nan
+    bad = [1, 4, 6, 8]
+    good = [i for i in range(rows) if i not in bad]
+    r2, h2 = ops.residual_norm(x2, y2, w, out_dtype=torch.float32, **kw)
+    r3, q, s = ops.residual_norm(x2, y2, w, out_dtype=torch.int8, **kw)
+    assert torch.equal(r2[good], r[good]) and torch.equal(h2[good], h[good])
+    assert torch.equal(r3[good], r[good]) and torch.isfinite(s[good]).all()
+    # an infinity or a NaN makes the layer norm's whole row NaN; in an RMS norm an infinite sum of
+    # squares makes the finite values 0
+    if norm == "layer":
+        assert torch.isnan(h2[bad]).all()
+    else:
+        assert not torch.isfinite(h2[bad]).all(-1).any()
+    assert int(q[bad].abs().max()) == 0 and not torch.isfinite(s[bad]).any()
+    if post is None:
+        assert torch.equal(r2[1, :3], r[1, :3]) and torch.isposinf(r2[1, 3]) and torch.isnan(r2[8, cols // 2])
