@@ -289,8 +289,8 @@ int m3r_match_nn_static(int device, const float* desc_1, const float* desc_2, in
 
 /* Rows in 8 bits:  a = max_j |x_ij|,  q_ij = the integer nearest to 127 x_ij / a (ties to
  * even, exact for every input),  scale_i = a / 127.  A row of zeros has scale 0; a row with an
- * infinity or a NaN holds zeros and that scale, so that products with it are NaN.
- * cols <= 16384. */
+ * infinity or a NaN holds zeros and that scale, so that products with it are NaN.  Rows below
+ * 1.5e-36 have a subnormal scale, with fewer bits.  cols <= 16384. */
 typedef struct m3r_quantize_args {
     int device;
     int dtype;           /* of x: M3R_DTYPE_BF16, _F16 or _F32 */
@@ -311,7 +311,8 @@ int m3r_quantize_rows(const m3r_quantize_args* args);
  * integers.  x in 16 or 32 bits is quantised row by row first (m3r_quantize_rows; k <= 16384)
  * into the workspace; x in 8 bits (rows 16-byte aligned, k <= 131071) comes with x_scale.
  * The weights' rows are 16-byte aligned: w a multiple of 16, ldw a multiple of 16 (pad the
- * rows of a k that is no multiple of 16; the padding is not used). */
+ * rows of a k that is no multiple of 16; the padding is not used).  Sum and scale_i are multiplied
+ * first, in 32 bits: rows of a magnitude above 3.4e38 / (127 k) may give infinities. */
 typedef struct m3r_int8_linear_args {
     int device;
     int x_dtype;         /* M3R_DTYPE_BF16, _F16, _F32 or _I8 */
@@ -374,7 +375,7 @@ int m3r_residual_norm(const m3r_residual_norm_args* args);
  *   (u, v) -> amplitude * (u cos a - v sin a, u sin a + v cos a),  a = position * inv_freq[i]
  * with pair i at (i, i + n_freq), or at (2 i, 2 i + 1) when interleaved; the values behind are
  * copied.  Positions are signed integers; angles are reduced in 64 bits, which leaves a position
- * of 2^31 its angle to 1e-6.  With axes = 2 (n_freq even) the first half of the pairs takes the
+ * of 2^31 its angle to 1e-6, and their sines and cosines are taken in 32.  With axes = 2 (n_freq even) the first half of the pairs takes the
  * positions of axis 0, the second those of axis 1.  out may be x itself, with the same strides. */
 typedef struct m3r_rope_tensor {
     const void* x;

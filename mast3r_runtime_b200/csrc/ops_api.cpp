@@ -14,7 +14,7 @@ void set_global_error(const std::string& msg);  // api.cpp: the text m3r_global_
 
 namespace {
 
-constexpr int64_t kMaxExtent = int64_t(1) << 40;  // no product of two sizes overflows 64 bits
+constexpr int64_t kMaxExtent = int64_t(1) << 40;  // row strides: past any device's memory
 
 template <class F>
 int guarded(F&& fn) {

@@ -13,7 +13,10 @@
 // many resident blocks hide the latency (2 or 4 accesses of a thread under way at once: 140
 // and 194 us instead of 130).  Angles are reduced in 64 bits -- position * (inv_freq / 2 pi)
 // minus its nearest integer -- so that a far position keeps its fraction of a turn: in 32
-// bits position 1e6 would leave it with 2^-5 of a radian.
+// bits position 1e6 would leave it with 2^-5 of a radian.  The fraction itself, its sine and
+// cosine and their product with the amplitude are 32-bit values: the error of 32-bit results is
+// 3.1e-8 to 5.7e-8 of them (root mean square, head sizes of 32 to 256), a quarter more on
+// average than with these in 64 bits (3.0e-8 to 4.2e-8).
 #include <algorithm>
 
 #include "common.cuh"

@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(LANES ? 128 : VEC ? 1024 : GT, row_blocks(VEC,
 
 // Many long rows: a block keeps its next rows of x and y on their way into shared memory with bulk
 // copies, so that the loads do not wait for the reductions of the row before and take no registers
-// (24,576 rows of 4,096, bf16: 129 us against 191; quantising alone gains nothing, 71 against 59).
+// (24,576 rows of 4,096, bf16: 133 us against 191; quantising alone gains nothing, 71 against 59).
 constexpr int kStreamStages = 4;
 
 __global__ void __launch_bounds__(1024) row_stream_kernel(const __grid_constant__ RowNormParams p, int stages) {
@@ -448,8 +448,10 @@ void launch(cudaStream_t s, const RowNormParams& p, int threads) {
 }
 
 // All of an SM's registers (64 a thread) in as many blocks as that makes, and shared memory but for
-// some that is left to L1, where the weight and gate vectors of every row come from (24,576 rows of
-// 4,096, bf16, with 225, 180 and 140 KB of rings: 133, 129, 128 us; 50,000 of 2,048: 134, 145, 142).
+// some that is left to L1, where the weight and gate vectors of every row come from (us with 225, 180 and
+// 140 KB of rings, 16-bit branch and result, one norm: 24,576 rows of 4,096, bf16 138, 133, 133, with two
+// norms and a gate 200, 186, 186; 50,000 of 2,048 137, 133, 146; 9,216 of 1,024 19.3, 17.5, 17.1.  Long 32-bit
+// rows would rather have two rows of ring than L1: 24,576 of 4,096 197, 207, 207; 12,288 of 8,192 191, 234, 234).
 // False where a block's share does not hold a row.
 bool launch_stream(cudaStream_t s, const RowNormParams& p, int threads) {
     constexpr int kMost = 180 * 1024;
@@ -477,6 +479,9 @@ bool aligned(const void* p, long long ld, int dt, int bytes) {
 // 17.5, 18.0 with a warp each; 32-bit stream, one norm: 6.9 and 6.6, 17.4, 17.8 and 19.3).  Of 768: 2,304
 // rows 6.1 with a block each, 4.8 with a warp, 4,608 9.9 and 9.2; 32-bit 5.8 and 5.1, 10.5 and 11.9.
 // More rows than that again are copied ahead (9,216 of 1,024, bf16: 23.7 and 22.7).
+// Of 264 to 512, one norm: 1,200 rows of 512 2.9 with a block each and 3.1 with a warp, 2,400 3.8 and 3.6,
+// 50,000 51.8 and 50.0; 32-bit 2,400 4.0 and 4.3, 50,000 53.0 and 51.7, of 320 44.2 and 40.5; quantised only, 600
+// rows 1.9 and 1.8, 2,300 3.1 and 2.2 (the one rule for both costs these 0.9 us), 9,216 10.2 and 4.1.
 // Quantised only: 300 rows of 1,024 1.7 us with a block each against 1.8, 1,000 2.6 against 1.9, 32-bit
 // 2.65 against 2.7; 2,300 of 768 3.3 against 2.9.
 void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
@@ -501,7 +506,10 @@ void dispatch_vec(cudaStream_t s, const RowNormParams& p) {
 // threads at neighbouring elements.  Threads without a value cost as much as the others, so the blocks
 // come in steps of a quarter to a half (24,576 rows of 513: 56 us in 128 threads, 44 in 96;
 // 5,000 of 5,003: 115 us with 8 values in 704 threads, which an SM holds once, 79 with 16 in 320; 9,000 of
-// 2,005, bf16 stream: 67 and 52; 4,039 of 1,001 with 16 values: 18.4 against 16.5).
+// 2,005, bf16 stream: 67 and 52; 4,039 of 1,001 with 16 values: 18.4 against 16.5).  They stay far from their
+// bytes' time (in us, that time behind the stroke): an access of 2 bytes a thread, and no rows copied ahead.
+// Norms, 16-bit branch and result: 24,576 of 513, bf16 42 / 15, 9,000 of 2,005 49 / 22, 40,001 of 129, 32-bit
+// 19 / 9.5, 9,000 of 3,333 80 / 55; quantised only, bf16: 24,576 of 513 16 / 5.8, 98,304 of 1,001 86 / 45.
 template <int NCH, int GT>
 void launch_elements(cudaStream_t s, const RowNormParams& p) {
     launch<false, NCH, 0, GT>(s, p, GT);

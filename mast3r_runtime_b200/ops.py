@@ -11,8 +11,10 @@ Tensors are torch CUDA tensors (this module is the only one of the package that 
 compiled side is binding/torch_ops.cpp).  A call runs on its tensors' device and on that device's
 current torch stream, queues its work without waiting, and can be captured into a CUDA graph; its
 results and workspace come from torch's allocator.  All tensors of a call are on one device, and the
-last dimension of the large ones is contiguous (other strides are free).  Bad arguments raise
-ValueError before anything is launched, device errors RuntimeError.  The operators have no
+last dimension of the large ones is contiguous; rope takes any other strides, the row operators rows
+that are evenly spaced.  Bad arguments raise ValueError before anything is launched, device errors
+RuntimeError, and a wait on the device that ran out is reported by status().  The calls are plain
+functions: torch.compile breaks its graph at each.  The operators have no
 gradients: the package runs models, it does not train them, and a call with a tensor that requires
 grad outside torch.no_grad(), or with one that carries a forward-mode tangent, is refused.
 """
@@ -39,8 +41,9 @@ def quantize_rows(x: torch.Tensor):
 
     With a = max |row|, q is the integer nearest to 127 x / a (ties to even) and scale = a / 127,
     so that q * scale is x to half a step.  A row of zeros has scale 0.  A row with an infinity
-    or a NaN holds zeros with an infinite or NaN scale: products with it are NaN.  q's rows lie
-    on 16-byte boundaries, as int8_linear needs them.  cols is at most 16,384."""
+    or a NaN holds zeros with an infinite or NaN scale: products with it are NaN.  Rows below 1.5e-36
+    have a subnormal scale, with fewer bits.  q's rows lie on 16-byte boundaries, as int8_linear
+    needs them.  cols is at most 16,384."""
     return _native.quantize_rows(x)
 
 
@@ -60,8 +63,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     comes with x_scale [...] (float32) and rows on 16-byte boundaries, as quantize_rows and
     residual_norm return them (k at most 131,071).  weight is int8 [n, k] with rows on 16-byte
     boundaries and weight_scale float32 [n], as quantize_weight returns them; bias float32 [n].
-    The sum over k is exact; scales, bias and activation ("none", "gelu" in its tanh form, "relu")
-    are applied in 32 bits and rounded once to out_dtype (default: x's type, bfloat16 for int8)."""
+    The sum over k is exact; scales (the row's first: rows above 3.4e38 / (127 k) may give infinities),
+    bias and activation ("none", "gelu" in its tanh form, "relu") are applied in 32 bits and rounded once
+    to out_dtype (default: x's type, bfloat16 for int8)."""
     return _native.int8_linear(x, weight, weight_scale, bias, act, out_dtype, x_scale)
 
 
@@ -130,7 +134,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     Pairs are (i, i + n), or (2 i, 2 i + 1) when interleaved.  positions are int32 or int64, [tokens]
     or [batch, tokens]; with axes = 2 ([2, tokens] or [2, batch, tokens]) the first half of the pairs
     turns with positions[0], the second with positions[1], as image tokens do with their row and
-    column.  inv_freq is float64 (rope_frequencies); angles are reduced in 64 bits.
+    column.  inv_freq is float64 (rope_frequencies); angles are reduced in 64 bits, their sines and
+    cosines taken in 32.
 
     Strides are free apart from the last dimension's (views of a packed projection).  Returns
     (q, k) turned: new tensors, q and k themselves with inplace, or the given out = (q_out, k_out)
