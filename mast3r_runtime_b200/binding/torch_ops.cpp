@@ -154,8 +154,10 @@ bool overlaps(const Tensor& a, const Tensor& b) {
 }
 
 bool same_view(const Tensor& a, const Tensor& b) {
-    return a.const_data_ptr() == b.const_data_ptr() && a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() &&
-           a.strides() == b.strides();
+    if (a.const_data_ptr() != b.const_data_ptr() || a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+    for (int64_t i = 0; i < a.dim(); ++i)
+        if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+    return true;
 }
 
 // A tensor that a call writes over: its version counts, and no element is there twice.

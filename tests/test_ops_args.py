@@ -367,3 +367,19 @@ def test_device_numbers_out_of_range_are_bad_arguments(device):
     from mast3r_runtime_b200 import _lib
 
     assert _lib.load().m3r_operator_status(device, None) == -1
+
+
+def test_the_same_view_by_other_strides_of_single_dimensions():
+    """Strides of dimensions of size 1 are of no meaning."""
+    from mast3r_runtime_b200 import ops
+
+    flat = torch.zeros(2, 24)
+    q = flat[:1].view(1, 1, 3, 8)
+    freq = torch.ones(4, dtype=torch.float64)
+    for strides in ((1, 24, 8, 1), (0, 0, 8, 1), (77, 5, 8, 1)):
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.rope(q, None, torch.zeros(1, dtype=torch.int64), freq, out=(q.as_strided(q.shape, strides), None))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.residual_norm(flat[:1], flat[:1].as_strided((1, 24), (3, 1)), None, inplace=True)
+    with pytest.raises(ValueError, match=SHARED):
+        ops.rope(q, None, torch.zeros(1, dtype=torch.int64), freq, out=(q.as_strided(q.shape, (0, 0, 8, 1), 1), None))
