@@ -23,8 +23,6 @@ int guarded(F&& fn) {
         m3r::set_global_error("");
         return M3R_OK;
     } catch (const m3r::Error& x) {
-        // the runtime keeps a failed call's error for the thread's next look: it is reported here
-        if (x.code == m3r::kErrCuda || x.code == m3r::kErrNoMem) cudaGetLastError();
         m3r::set_global_error(x.what());
         return x.code;
     } catch (const std::bad_alloc&) {

@@ -28,13 +28,17 @@ constexpr int kErrTimeout = -5;
 constexpr int kErrState = -6;
 constexpr int kErrNoMem = -7;
 
+// The runtime also keeps a failed call's error for the thread's next cudaGetLastError, where a later, good
+// launch would find it: it is reported here and taken back.
 #define M3R_CUDA(call)                                                                                 \
     do {                                                                                               \
         cudaError_t e_ = (call);                                                                       \
-        if (e_ != cudaSuccess)                                                                         \
+        if (e_ != cudaSuccess) {                                                                       \
+            cudaGetLastError();                                                                        \
             throw ::m3r::Error(e_ == cudaErrorMemoryAllocation ? ::m3r::kErrNoMem : ::m3r::kErrCuda,   \
                                std::string(#call) + ": " + cudaGetErrorString(e_) + " (" + __FILE__ + \
                                    ":" + std::to_string(__LINE__) + ")");                              \
+        }                                                                                              \
     } while (0)
 
 #define M3R_REQUIRE(cond, msg)                                            \
