@@ -1,6 +1,6 @@
 """GPU tests of the operators at the edges of their ranges: results far below the values they are
-made from, columns and rows that are not finite, heads and head
-counts past a block's share, errors of one call that must not show in the next.
+made from, columns and rows that are not finite, heads and head counts past a block's share, errors
+of one call that must not show in the next, waits that run out.
 
 Tolerances count roundings as test_gpu_ops.py does: U = 2^-24 is one 32-bit rounding, half(dtype)
 half a step of the result's type."""
